@@ -48,8 +48,8 @@ enum {
   TSDS_E_DEVICE = 7,      /* device query failed / not an sm_100 device */
   TSDS_E_SCRATCH_LIMIT = 8, /* request larger than a built-in scratch area */
   TSDS_E_RUNTIME = 9,       /* a CUDA runtime call (allocation, IPC mapping) failed */
-  TSDS_E_INDEX = 10         /* a device-side table entry (KV pool row) outside its pool:
-                               the access was redirected to row 0 (status word) */
+  TSDS_E_INDEX = 10         /* a device-side index outside its range (status word): a KV pool row
+                               (the access was redirected to row 0) or an adapter (none applied) */
 };
 
 /* Human-readable name of a status code (static string). */
@@ -209,6 +209,72 @@ int tsds_linear_f32(const void* x, int ldx, const void* W, float* out, int ldo, 
 int tsds_linear_bias(const void* x, int ldx, const void* W, const void* bias, void* out, int ldo,
                      int M, int n_out, int K, void* workspace, size_t workspace_bytes,
                      tsds_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit projections with per-request adapters.  No counterpart in the
+ * reference (its projections are bf16 and shared by every request): a
+ * decoder layer over e4m3 weights (a scale per output channel) and e4m3
+ * activations (a scale per token row), the adapters in bf16.
+ *
+ * tsds_quant_fp8: rows to e4m3.  s = max(max_k |x[k]|, 2^-100) / 448,
+ *   q[k] = e4m3(x[k] / s), to nearest even; scale[row] = s.  Quantises a
+ *   projection's weights (row = output channel) and the activations that no
+ *   norm precedes (attention output, SwiGLU output).  A row that holds a NaN
+ *   or an infinity gets a NaN or infinite scale and NaN values.
+ * x: [rows][n] bf16, row stride ldx; q: [rows][n] bytes, row stride ldq;
+ * n % 16 == 0, ldx % 8 == 0, ldq % 16 == 0, x and q 16-byte aligned.
+ * rows == 0 is allowed here and below (nothing is launched).
+ */
+int tsds_quant_fp8(const void* x, void* q, float* scale, int rows, int n, int ldx, int ldq,
+                   tsds_stream_t stream);
+/* Residual addition + RMSNorm + e4m3 in one pass over the rows:
+ *   r = bf16(x + res)                    stored to res_out (the residual stream)
+ *   y = r * rsqrt(mean(r^2) + eps) * w   fp32, not rounded
+ *   (q, scale) = the row quantisation of y as above
+ *   norm_out = bf16(y)                   optional: what adapters beside the projection read
+ * res NULL: r = x, res_out unused.  res_out (row stride ld_res_out) may be
+ * res or x itself, with its row stride: the update in place.  Other overlaps
+ * are not allowed.  Same alignment rules as above. */
+int tsds_add_rms_norm_fp8(const void* x, const void* res, const void* w, void* res_out, void* q,
+                          float* scale, void* norm_out, int rows, int n, int ldx, int ld_res,
+                          int ld_res_out, int ldq, int ld_norm, float eps, tsds_stream_t stream);
+/* acc[m][j] = (sum_k W[j][k] x[m][k]) * x_scale[m] * w_scale[j] in fp32, then
+ *   tsds_linear_fp8:           out = bf16(acc)
+ *   tsds_linear_residual_fp8:  out = bf16(res + acc)      (out may be res)
+ *   tsds_linear_swiglu_fp8:    W = [gate; up] ([2*n_out][K], 2*n_out scales);
+ *                              out = bf16(silu(acc_gate) * acc_up)
+ * rounded once.  x: [M][K] e4m3 bytes (row stride ldx, ldx % 16 == 0), W
+ * [n_out][K] e4m3 contiguous, K % 16 == 0, x and W 16-byte aligned; any M
+ * and n_out.  tcgen05 tensor cores; no workspace.  *status (device int32,
+ * zero before the first use): TSDS_E_TIMEOUT if a device wait gave up
+ * (tsds_set_wait_limit_ns). */
+int tsds_linear_fp8(const void* x, int ldx, const float* x_scale, const void* W, const float* w_scale,
+                    void* out, int ldo, int M, int n_out, int K, int32_t* status, tsds_stream_t stream);
+int tsds_linear_residual_fp8(const void* x, int ldx, const float* x_scale, const void* W,
+                             const float* w_scale, const void* res, int res_ld, void* out, int ldo, int M,
+                             int n_out, int K, int32_t* status, tsds_stream_t stream);
+int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const void* W,
+                           const float* w_scale, void* out, int ldo, int M, int n_out, int K,
+                           int32_t* status, tsds_stream_t stream);
+/* Low-rank adapters of many requests added to a projection's output y [M][N]
+ * (row m uses adapter a = adapter[m]; a < 0: none, out = y):
+ *   out[m][j] = bf16(y[m][j] + scale[a] * sum_{r < ranks[a]} B[a][j][r] *
+ *                    sum_k A[a][s(j)*R + r][k] * x[m][k])
+ * x: [M][K] bf16, A: [n_adapters][n_slices*R][K], B: [n_adapters][N][R],
+ * contiguous.  n_slices projections side by side in y's columns (q, k, v:
+ * 3): slice_widths (host array, each a multiple of 32, summing to N) gives
+ * the columns of each, s(j) is column j's; NULL with one slice.  scale
+ * (fp32) and ranks (int32, what an adapter uses of R; the rest of its A and
+ * B is not part of the sum, whatever it holds) may be NULL: 1 and R.
+ * out may be y (ldo == ldy; rows without an adapter are then not touched).
+ * Any order of adapters; rows of one request next to one another are
+ * fastest.  K % 8 == 0, N % 8 == 0, R % 8 == 0, R <= 128, n_slices <= 4;
+ * strides multiples of 8, buffers 16-byte aligned.  An adapter[m] >= n_adapters is not
+ * followed: the row is treated as one without and *status = TSDS_E_INDEX. */
+int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, const void* lora_a, const void* lora_b,
+                  const int32_t* adapter, const float* scale, const int32_t* ranks, void* out, int ldo,
+                  int M, int K, int N, int n_adapters, int R, int n_slices, const int32_t* slice_widths,
+                  int32_t* status, tsds_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Verify / decode attention of T new tokens per sequence over the KV cache.

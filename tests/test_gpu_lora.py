@@ -1,0 +1,151 @@
+"""GPU checks of the per-request low-rank adapters against their definition in 64 bits."""
+import pytest
+import torch
+
+import fp8_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tri_sds_b200 import ops as o
+    yield o
+    o.check_status()
+
+
+def _case(M, K, slices, R, n_ad, adapters, seed=0, scale=True, ranks=True):
+    g = torch.Generator(device=DEV).manual_seed(seed + M + K + R)
+
+    def rnd(*shape, std=1.0):
+        return (torch.randn(*shape, device=DEV, generator=g) * std).to(BF)
+
+    N = sum(slices)
+    st = dict(y=rnd(M, N), x=rnd(M, K), lora_a=rnd(n_ad, len(slices) * R, K, std=K ** -0.5),
+              lora_b=rnd(n_ad, N, R, std=0.1), adapter=torch.tensor(adapters, dtype=torch.int32, device=DEV),
+              slices=slices if len(slices) > 1 else None)
+    st["scale"] = torch.rand(n_ad, device=DEV, generator=g) + 0.5 if scale else None
+    st["ranks"] = torch.tensor([max(1, R - 3 * i) for i in range(n_ad)], dtype=torch.int32, device=DEV) \
+        if ranks else None
+    return st
+
+
+def _check(ops, st, out=None):
+    want, err = ref.lora(st["y"], st["x"], st["lora_a"], st["lora_b"], st["adapter"], st["scale"], st["ranks"],
+                         st["slices"])
+    got = ops.lora_add(out=out, **st)
+    ref.check_bf16(got, want, err)
+    none = st["adapter"] < 0
+    assert torch.equal(got[none], st["y"][none]) if out is not st["y"] else True
+    return got
+
+
+@pytest.mark.parametrize("M,K,slices,R,n_ad", [
+    (1, 8, [8], 8, 1), (1, 5120, [1024, 128, 128], 16, 2), (8, 5120, [8192, 1024, 1024], 16, 8), (3, 40, [200], 24, 4),
+    (16, 264, [32, 64, 96, 32], 128, 2), (17, 1000, [1000], 48, 3), (26, 2560, [2560], 64, 1), (100, 512, [96, 32], 8, 16),
+    (208, 25600, [5120], 64, 8), (1024, 128, [256], 16, 5), (1025, 136, [264], 24, 5), (1500, 640, [640, 128, 128], 32, 4),
+    (2100, 72, [96, 96], 128, 3)])
+@pytest.mark.parametrize("order", ["runs", "scattered"])
+def test_lora(ops, M, K, slices, R, n_ad, order):
+    if order == "runs":      # requests of 5 rows each, every (n_ad + 1)-th without an adapter
+        ad = [(m // 5) % (n_ad + 1) - 1 for m in range(M)]
+    else:
+        g = torch.Generator().manual_seed(M)
+        ad = torch.randint(-1, n_ad, (M,), generator=g).tolist()
+    _check(ops, _case(M, K, slices, R, n_ad, ad))
+
+
+@pytest.mark.parametrize("M", [40, 1400])
+def test_lora_in_place_leaves_other_rows_alone(ops, M):
+    st = _case(M, 320, [288, 64], 16, 3, [(m % 4) - 1 for m in range(M)])
+    want = _check(ops, st)
+    y = st["y"].clone()
+    st["y"] = y
+    got = ops.lora_add(out=y, **st)
+    assert got is y and torch.equal(got, want)
+
+
+def test_lora_without_scale_and_ranks(ops):
+    _check(ops, _case(19, 512, [512], 32, 4, [m % 4 for m in range(19)], scale=False, ranks=False))
+
+
+def test_lora_unused_ranks_are_not_read_into_the_sum(ops):
+    """NaN past an adapter's rank (in A's rows and in B's columns) changes nothing."""
+    for R, used in [(16, 1), (24, 7), (64, 33), (32, 0), (128, 66)]:
+        st = _case(21, 264, [96, 160], R, 2, [m % 2 for m in range(21)])
+        st["ranks"] = torch.tensor([used, R], dtype=torch.int32, device=DEV)
+        for s in range(2):
+            st["lora_a"][0, s * R + used:(s + 1) * R] = float("nan")
+        st["lora_b"][0, :, used:] = float("inf")
+        _check(ops, st)
+
+
+def test_lora_ranks_out_of_range_are_clamped(ops):
+    st = _case(5, 64, [64], 16, 2, [0, 1, 0, 1, -1])
+    full = dict(st, ranks=torch.tensor([16, 0], dtype=torch.int32, device=DEV))
+    wild = dict(st, ranks=torch.tensor([1000, -5], dtype=torch.int32, device=DEV))
+    assert torch.equal(ops.lora_add(**full), ops.lora_add(**wild))
+
+
+@pytest.mark.parametrize("M", [33, 1300])
+def test_lora_index_past_the_last_adapter_is_reported(ops, M):
+    ids = [m % 3 for m in range(M)]
+    ids[7] = 3
+    ids[20] = 2 ** 31 - 1
+    st = _case(M, 128, [128], 16, 3, ids)
+    got = ops.lora_add(**st)
+    assert torch.equal(got[7], st["y"][7]) and torch.equal(got[20], st["y"][20])
+    with pytest.raises(RuntimeError, match="status 10"):
+        ops.check_status()
+    want, err = ref.lora(st["y"], st["x"], st["lora_a"], st["lora_b"], st["adapter"], st["scale"], st["ranks"], None)
+    ref.check_bf16(got, want, err)
+
+
+def test_lora_strides_and_neighbours(ops):
+    g = torch.Generator(device=DEV).manual_seed(2)
+    st = _case(30, 256, [128, 64], 16, 3, [(m // 7) - 1 for m in range(30)])
+    wide_x = torch.randn(30, 400, device=DEV, generator=g).to(BF)
+    st["x"] = wide_x[:, 64:320]
+    wide_y = torch.randn(30, 256, device=DEV, generator=g).to(BF)
+    st["y"] = wide_y[:, 32:224]
+    buf = torch.full((32, 264), 5.0, device=DEV, dtype=BF)
+    _check(ops, st, out=buf[1:31, 8:200])
+    keep = torch.ones_like(buf, dtype=torch.bool)
+    keep[1:31, 8:200] = False
+    assert (buf[keep] == 5).all()
+    with pytest.raises(RuntimeError, match="status 10"):   # rows 28 and 29 name adapter 3 of 3
+        ops.check_status()
+
+
+def test_lora_nothing_to_add(ops):
+    st = _case(40, 128, [128], 16, 2, [-1] * 40)
+    assert torch.equal(ops.lora_add(**st), st["y"])
+    y = st["y"].clone()
+    assert torch.equal(ops.lora_add(**dict(st, y=y, out=y)), st["y"])
+    e = _case(0, 128, [128], 16, 2, [])
+    assert ops.lora_add(**e).shape == (0, 128)
+
+
+def test_lora_same_bits_every_time(ops):
+    st = _case(208, 5120, [1024], 64, 8, [m // 26 for m in range(208)])
+    first = ops.lora_add(**st)
+    for _ in range(20):
+        assert torch.equal(first, ops.lora_add(**st))
+
+
+def test_lora_offsets_past_32_bits(ops):
+    """An adapter whose rows lie past 2^31 elements of lora_a."""
+    K, R, n_ad = 4096, 64, 8200
+    a = torch.zeros(n_ad, R, K, device=DEV, dtype=BF)
+    assert a.numel() > 2 ** 31
+    st = _case(6, K, [64], R, 1, [0] * 6, ranks=False)
+    want = ops.lora_add(**st)
+    a[-1] = st["lora_a"][0]
+    b = torch.zeros(n_ad, 64, R, device=DEV, dtype=BF)
+    b[-1] = st["lora_b"][0]
+    scale = torch.ones(n_ad, device=DEV)
+    scale[-1] = st["scale"][0]
+    got = ops.lora_add(st["y"], st["x"], a, b, torch.full((6,), n_ad - 1, dtype=torch.int32, device=DEV), scale=scale)
+    assert torch.equal(got, want)

@@ -75,6 +75,12 @@ SIGNATURES = {
     "tsds_linear_residual_norm": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _F, _P, _Z, _P]),
     "tsds_linear_swiglu": (_I, [_P, _I, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
     "tsds_linear_bias": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
+    "tsds_quant_fp8": (_I, [_P, _P, _P, _I, _I, _I, _I, _P]),
+    "tsds_add_rms_norm_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "tsds_linear_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "tsds_linear_residual_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P]),
+    "tsds_linear_swiglu_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "tsds_lora_add": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "tsds_logits_topk": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P]),
     "tsds_tree_state_bytes": (_Z, [_I]),
     "tsds_tree_init": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),

@@ -27,9 +27,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 load_encode_tiled() {
   return f;
 }
 
-int tsds_make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
-                           uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
-                           int swizzle_128b) {
+static int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                        uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle_128b) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = load_encode_tiled();
   if (!encode) return TSDS_E_DEVICE;
   if (!tsds_aligned16(base) || (row_stride_bytes % 16) != 0) return TSDS_E_ALIGN;
@@ -37,11 +36,24 @@ int tsds_make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, u
   cuuint64_t strides[1] = {row_stride_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
+  CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides,
                               box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               swizzle_128b ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? TSDS_OK : TSDS_E_INVALID;
+}
+
+int tsds_make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                           uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
+                           int swizzle_128b) {
+  return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, inner, outer, row_stride_bytes, box_inner,
+                      box_outer, swizzle_128b);
+}
+
+int tsds_make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                         uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+  return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_stride_bytes, box_inner, box_outer,
+                      1);
 }
 
 extern "C" const char* tsds_status_string(int status) {
@@ -56,7 +68,7 @@ extern "C" const char* tsds_status_string(int status) {
     case TSDS_E_DEVICE: return "device / driver query failed";
     case TSDS_E_SCRATCH_LIMIT: return "request larger than the built-in scratch area";
     case TSDS_E_RUNTIME: return "CUDA runtime call (allocation / IPC) failed";
-    case TSDS_E_INDEX: return "KV pool row outside the pool (table entry)";
+    case TSDS_E_INDEX: return "device-side index (KV pool row, adapter) out of range";
     default: return "unknown status";
   }
 }

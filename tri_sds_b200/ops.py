@@ -403,3 +403,165 @@ def accept_greedy(draft: torch.Tensor, target: torch.Tensor, target_len: torch.T
     _lib.call("tsds_accept_greedy", _p(draft), _p(target), _p(acc), _p(tokens), _p(target_len), _p(last), _p(cur),
               B, K, _stream())
     return acc, tokens
+
+
+# -- 8-bit projections with per-request adapters ------------------------------
+
+FP8 = torch.float8_e4m3fn
+
+
+def _on(device, name: str, *args) -> None:
+    """_lib.call on `device`'s current stream; the tensors need not be on the
+    current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream())
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, _stream())
+
+
+def _one_device(t, *ts):
+    """The device of all the tensors given."""
+    for o in ts:
+        _need(o is None or o.device == t.device, "tensors on different devices")
+    return t.device
+
+
+def _rows(t, n: int, what: str):
+    """A 2-D row buffer of `n` columns with unit inner stride: its row stride
+    (of one row: n, whatever torch keeps there)."""
+    _need(t.dim() == 2 and t.shape[1] == n and (n == 1 or t.stride(1) == 1),
+          f"{what} must be [rows, {n}] with unit inner stride")
+    return t.stride(0) if t.shape[0] > 1 else n
+
+
+def quant_fp8(x: torch.Tensor, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """Rows of x [rows, n] bf16 to e4m3: (q [rows, n] float8_e4m3fn, scale
+    [rows] fp32) with scale = max|x| / 448 of the row, q = e4m3(x / scale).
+    Weights ([out, in]: a scale per output channel) as well as activations."""
+    _bf16_cuda(x)
+    _cuda(FP8, out)
+    _cuda(torch.float32, scale)
+    _need(x.dim() == 2, "x must be [rows, n]")
+    rows, n = x.shape
+    out = torch.empty(rows, n, dtype=FP8, device=x.device) if out is None else out
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device) if scale is None else scale
+    dev = _one_device(x, out, scale)
+    _need(out.shape[0] == rows and scale.shape == (rows,) and scale.is_contiguous(), "out / scale mismatch")
+    _on(dev, "tsds_quant_fp8", _p(x), _p(out), _p(scale), rows, n, _rows(x, n, "x"), _rows(out, n, "out"))
+    return out, scale
+
+
+def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                     out: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                     res_out: torch.Tensor | None = None, norm_out: torch.Tensor | None = None):
+    """r = bf16(x + residual), y = RMSNorm(r) * weight, y's rows to e4m3, in
+    one launch: (q [rows, n] float8_e4m3fn, scale [rows] fp32, res_out [rows,
+    n] bf16).  res_out may be the residual itself (the update in place).
+    Without a residual r = x and res_out is None.  norm_out, when given,
+    receives y in bf16 (what per-request adapters read, see lora_add)."""
+    _bf16_cuda(x, weight, residual, res_out, norm_out)
+    _cuda(FP8, out)
+    _cuda(torch.float32, scale)
+    _need(x.dim() == 2, "x must be [rows, n]")
+    rows, n = x.shape
+    _need(weight.shape == (n,) and weight.is_contiguous(), "weight must be [n]")
+    _need(residual is not None or res_out is None, "res_out without a residual")
+    out = torch.empty(rows, n, dtype=FP8, device=x.device) if out is None else out
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device) if scale is None else scale
+    if residual is not None and res_out is None:
+        res_out = torch.empty(rows, n, dtype=x.dtype, device=x.device)
+    dev = _one_device(x, weight, residual, out, scale, res_out, norm_out)
+    for t in (residual, out, res_out, norm_out):
+        _need(t is None or t.shape == (rows, n), "shape mismatch")
+    _need(scale.shape == (rows,) and scale.is_contiguous(), "scale must be [rows]")
+    ld_res, ld_out = (n, n) if residual is None else (_rows(residual, n, "residual"), _rows(res_out, n, "res_out"))
+    _on(dev, "tsds_add_rms_norm_fp8", _p(x), _p(residual), _p(weight), _p(res_out), _p(out), _p(scale), _p(norm_out),
+        rows, n, _rows(x, n, "x"), ld_res, ld_out, _rows(out, n, "out"),
+        n if norm_out is None else _rows(norm_out, n, "norm_out"), float(eps))
+    return out, scale, res_out
+
+
+def _fp8_operands(x, x_scale, w, w_scale, n_out, out):
+    """Checks of the 8-bit projections; returns (M, K, out)."""
+    _cuda(FP8, x, w)
+    _cuda(torch.float32, x_scale, w_scale)
+    _bf16_cuda(out)
+    _need(x.dim() == 2 and w.dim() == 2, "x must be [M, K] and w [out, K]")
+    M, K = x.shape
+    _need(w.shape[1] == K and w.is_contiguous(), "w must be contiguous [out, K]")
+    _need(x_scale.shape == (M,) and x_scale.is_contiguous(), "x_scale must be [M]")
+    _need(w_scale.shape == (w.shape[0],) and w_scale.is_contiguous(), "w_scale must hold a scale per row of w")
+    out = torch.empty(M, n_out, dtype=torch.bfloat16, device=x.device) if out is None else out
+    _need(out.shape == (M, n_out), "out must be [M, out]")
+    return M, K, out
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               out: torch.Tensor | None = None):
+    """(x * x_scale) @ (w * w_scale)^T -> bf16 [M, n_out] for e4m3 x [M, K]
+    (a scale per row) and w [n_out, K] (a scale per output channel)."""
+    n_out = w.shape[0]
+    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
+    dev = _one_device(x, x_scale, w, w_scale, out)
+    _on(dev, "tsds_linear_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(out),
+        _rows(out, n_out, "out"), M, n_out, K, _p(_scratch.status_word(dev)))
+    return out
+
+
+def linear_residual_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                        res: torch.Tensor, out: torch.Tensor | None = None):
+    """res + the 8-bit projection of linear_fp8, rounded once; out may be res."""
+    n_out = w.shape[0]
+    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
+    _bf16_cuda(res)
+    _need(res.shape == (M, n_out), "res must be [M, n_out]")
+    dev = _one_device(x, x_scale, w, w_scale, out, res)
+    _on(dev, "tsds_linear_residual_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(res),
+        _rows(res, n_out, "res"), _p(out), _rows(out, n_out, "out"), M, n_out, K, _p(_scratch.status_word(dev)))
+    return out
+
+
+def linear_swiglu_fp8(x: torch.Tensor, x_scale: torch.Tensor, w_gate_up: torch.Tensor, w_scale: torch.Tensor,
+                      out: torch.Tensor | None = None):
+    """silu(gate) * up of the 8-bit projections for w_gate_up = [gate; up]
+    ([2I, K] e4m3, 2I scales) -> bf16 [M, I], rounded once."""
+    _need(w_gate_up.shape[0] % 2 == 0, "w_gate_up must be [2I, K]")
+    I = w_gate_up.shape[0] // 2
+    M, K, out = _fp8_operands(x, x_scale, w_gate_up, w_scale, I, out)
+    dev = _one_device(x, x_scale, w_gate_up, w_scale, out)
+    _on(dev, "tsds_linear_swiglu_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(out),
+        _rows(out, I, "out"), M, I, K, _p(_scratch.status_word(dev)))
+    return out
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, adapter: torch.Tensor,
+             scale: torch.Tensor | None = None, ranks: torch.Tensor | None = None,
+             slices: list[int] | None = None, out: torch.Tensor | None = None):
+    """The low-rank adapters of many requests added to a shared projection's
+    output: out[m] = y[m] + scale[a] * B_a (A_a x[m]) with a = adapter[m]
+    (int32 [M]; negative: none).  y [M, N], x [M, K] bf16; lora_a
+    [adapters, S * R, K], lora_b [adapters, N, R] bf16; ``slices``: the column
+    widths of S projections side by side in y (q, k, v), each with its own R
+    rows of lora_a; ``ranks`` (int32): what each adapter uses of R; ``scale``
+    fp32, default 1.  out may be y (in place).  An index past the last adapter
+    leaves the row as it is and is reported by check_status()."""
+    _bf16_cuda(y, x, lora_a, lora_b, out)
+    _cuda(torch.int32, adapter, ranks)
+    _cuda(torch.float32, scale)
+    _need(y.dim() == 2 and x.dim() == 2 and lora_a.dim() == 3 and lora_b.dim() == 3, "bad dimensions")
+    (M, N), K = y.shape, x.shape[1]
+    n_ad, R, S = lora_a.shape[0], lora_b.shape[2], 1 if slices is None else len(slices)
+    _need(x.shape[0] == M and lora_a.shape == (n_ad, S * R, K) and lora_b.shape == (n_ad, N, R), "shape mismatch")
+    _need(lora_a.is_contiguous() and lora_b.is_contiguous(), "lora_a and lora_b must be contiguous")
+    _need(adapter.shape == (M,) and adapter.is_contiguous(), "adapter must be [M]")
+    for t in (scale, ranks):
+        _need(t is None or (t.shape == (n_ad,) and t.is_contiguous()), "scale and ranks hold a value per adapter")
+    out = torch.empty(M, N, dtype=y.dtype, device=y.device) if out is None else out
+    _need(out.shape == y.shape, "out must have y's shape")
+    dev = _one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out)
+    widths = None if slices is None else (ctypes.c_int32 * S)(*slices)
+    _on(dev, "tsds_lora_add", _p(y), _rows(y, N, "y"), _p(x), _rows(x, K, "x"), _p(lora_a), _p(lora_b), _p(adapter),
+        _p(scale), _p(ranks), _p(out), _rows(out, N, "out"), M, K, N, n_ad, R, S, widths,
+        _p(_scratch.status_word(dev)))
+    return out
