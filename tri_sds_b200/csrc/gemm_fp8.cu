@@ -4,22 +4,26 @@
 //   out[m][j] = epilogue( (sum_k W[j][k] X[m][k]) * sx[m] * sw[j] )
 //
 // Weight rows j fill the MMA's M = 128, token rows m are its N (at most 256
-// per block), K goes in blocks of 128 bytes.  Few token rows make the
-// weights' bytes the cost, so they have to stream through every SM at once:
-// a weight tile's K range is split over a cluster of C CTAs, C as large as
-// keeps all CTAs of the launch resident.  Each CTA sums its share in TMEM; at
-// the end every CTA stores its fp32 partial in its own shared memory and, after
-// one cluster barrier, finishes 1/C of the tile from all C partials, read
-// over distributed shared memory in rank order.  No partial goes through
-// global memory, there is no workspace, no counter and no atomic, and the
-// result of a call is always the same bits.
+// per block), K goes in blocks of 128 bytes.  A unit is one weight tile times
+// one token block; two schedules, by the number of units:
+//
+// * Few units (at most the CTAs that are resident at once): a unit's K range is
+//   split over a cluster of C CTAs, C as large as keeps the launch resident, so
+//   that the weights stream through every SM at once.  Each CTA sums its share
+//   in TMEM; at the end every CTA stores its fp32 partial in its own shared
+//   memory and, after one cluster barrier, finishes 1/C of the token rows
+//   from all C partials, read over distributed shared memory in rank order.
+//   No partial goes through global memory, there is no workspace, no counter
+//   and no atomic, and a call always gives the same bits.
+// * Many units: persistent CTAs take whole units in turn (C = 1) with two
+//   accumulators in TMEM, so the epilogue of one unit runs under the main
+//   loop of the next and the ring never drains.
 //
 // Warp 0 requests the tiles (TMA, 128-byte swizzle), warp 1 issues
-// tcgen05.mma kind::f8f6f4 (fp32 accumulators in TMEM), warps 2-5 move the
-// accumulators to shared memory; all six finish the outputs.  Before the
-// dependency wait the first weight tiles are only prefetched into L2: the
-// weights may come from an earlier kernel of the stream (tsds_quant_fp8), so
-// they are read after it.
+// tcgen05.mma kind::f8f6f4 (fp32 accumulators in TMEM), warps 2-5 drain the
+// accumulators.  Before the dependency wait the first weight tiles are only
+// prefetched into L2: the weights may come from an earlier kernel of the
+// stream (tsds_quant_fp8), so they are read after it.
 // Every mbarrier wait is bounded; a CTA that gives up records TSDS_E_TIMEOUT
 // and still takes part in the cluster's barriers.
 #include "common.cuh"
@@ -39,11 +43,14 @@ constexpr int RING = 8;                  // most stages
 constexpr int MAX_C = 8;                 // largest portable cluster
 constexpr int SMEM_SM = 233472;          // 228 KB per SM
 constexpr int SMEM_CTA = 220 * 1024;     // dynamic shared memory a CTA may ask for
+constexpr int STAGING = 2 * 16 * TILE_J * 4;   // output staging of a persistent CTA
 constexpr int SMEM_SIDE = 2048;          // static shared memory + the system's 1 KB per CTA
 
 struct F8Args {
   int M, n_out, KT, C, blocks;  // blocks of MAX_ROWS token rows
+  int units, bufs;              // units of the launch; accumulators per CTA
   int npad, stages, b_bytes, chunk;
+  int out_off;                  // C == 1: offset of the output staging (0: the ring, free by then)
   int ldo, res_ld;
   const float *sx, *sw;
   const bf16* res;
@@ -55,7 +62,7 @@ struct F8Args {
 };
 
 struct F8Shared {
-  uint64_t full[RING], empty[RING], done, drain;
+  uint64_t full[RING], empty[RING], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
 };
@@ -65,6 +72,17 @@ __device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// a bounded wait of a whole warp, with one outcome for all its lanes
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase, limit_ns));
 }
 
 __device__ __forceinline__ float4 ld_peer(uint32_t addr) {
@@ -77,16 +95,24 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
-// every thread of the cluster (or of the CTA, when it is alone)
-__device__ __forceinline__ void unit_barrier(int C) {
+__device__ __forceinline__ void cluster_barrier() {
   __syncwarp();
-  if (C > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
+  cluster_sync_all();
 }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+// whether `ok` holds in all 128 threads of the epilogue warps
+__device__ __forceinline__ bool epi_all(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.red.and.pred q, 1, 128, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
 template <int EPI>
 __global__ void __launch_bounds__(THREADS)
@@ -95,26 +121,31 @@ __global__ void __launch_bounds__(THREADS)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ F8Shared sh;
   constexpr bool SW = EPI == EPI_SWIGLU;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = p.C > 1 ? (int)cluster_ctarank() : 0;
-  const int unit = blockIdx.x / p.C;            // (weight tile, token block), token blocks fastest:
-  const int tile = unit / p.blocks;             // the tiles in flight share their weights through L2
-  const int m_base = (unit - tile * p.blocks) * MAX_ROWS;
+  const int first_unit = blockIdx.x / p.C, unit_step = gridDim.x / p.C;
   const int k_lo = rank * p.KT / p.C, nk = (rank + 1) * p.KT / p.C - k_lo;
+  // unit -> weight tile and first token row; token blocks fastest, so that the
+  // units in flight share their weights through L2
+  auto tile_of = [&](int u) { return u / p.blocks; };
+  auto row_of = [&](int u) { return (u - u / p.blocks * p.blocks) * MAX_ROWS; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&sh.full[s], 1);
       mbar_init(&sh.empty[s], 1);
     }
-    mbar_init(&sh.done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.tfull[i], 1);
+      mbar_init(&sh.tempty[i], 4);   // one arrival per epilogue warp
+    }
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(p.tmem_cols));
+                 "r"(p.bufs * p.tmem_cols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
@@ -125,66 +156,209 @@ __global__ void __launch_bounds__(THREADS)
   uint8_t* b_smem = smem + p.stages * A_BYTES;
   pdl_trigger();
   int issued = 0;
-  // a stage's weight rows: 128 of one matrix, or 64 gate and 64 up rows
-  const int row0 = SW ? tile * 64 : tile * TILE_J;
-  const int row1 = SW ? p.n_out + tile * 64 : row0 + 64;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      prefetch_tmap(&amap);
-      prefetch_tmap(&bmap);
-      for (int i = 0; i < nk && i < p.stages; ++i) {
-        tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, row0);
-        tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, row1);
-      }
-      pdl_wait();
-      for (int i = 0; i < nk; ++i) {
-        const int s = i % p.stages;
-        if (i >= p.stages && !mbar_wait(&sh.empty[s], (i / p.stages - 1) & 1, p.wait_ns)) {
-          atomicExch(p.status, TSDS_E_TIMEOUT);
-          *(volatile int*)&sh.abort = 1;
-          break;
-        }
-        mbar_arrive_expect_tx(&sh.full[s], A_BYTES + p.b_bytes);
-        const int x = (k_lo + i) * KB;
-        tma_load_2d(a_smem + s * A_BYTES, &amap, &sh.full[s], x, row0);
-        tma_load_2d(a_smem + s * A_BYTES + A_BYTES / 2, &amap, &sh.full[s], x, row1);
-        tma_load_2d(b_smem + s * p.b_bytes, &bmap, &sh.full[s], x, m_base);
-        issued = i + 1;
+  // what a thread of the epilogue works on: four channels j .. j+3 of the tile
+  // (their scales in registers) and every token row that is its turn
+  constexpr int G = SW ? 16 : 32;
+  struct Out {
+    int j, left;      // first channel; channels inside the output
+    bool vec;         // 8-byte accesses
+    float sw[SW ? 2 : 1][4];
+  };
+  auto out_of = [&](int tile, int g4) {
+    Out w;
+    w.j = (SW ? tile * 64 : tile * TILE_J) + g4;
+    w.left = p.n_out - w.j;
+    w.vec = w.left >= 4 && (p.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 &&
+            (EPI != EPI_RESIDUAL || ((p.res_ld % 4) == 0 && (reinterpret_cast<uintptr_t>(p.res) & 7) == 0));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w.sw[0][i] = i < w.left ? p.sw[w.j + i] : 0.f;
+      if constexpr (SW) w.sw[1][i] = i < w.left ? p.sw[p.n_out + w.j + i] : 0.f;
+    }
+    return w;
+  };
+  auto finish = [&](const Out& w, int m, const float4 (&acc)[2]) {
+    const float sx = p.sx[m];
+    const float a4[4] = {acc[0].x, acc[0].y, acc[0].z, acc[0].w};
+    float rv[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+    if constexpr (EPI == EPI_RESIDUAL) {
+      const bf16* rp = p.res + (int64_t)m * p.res_ld + w.j;
+      if (w.vec) {
+        const uint2 u = *reinterpret_cast<const uint2*>(rp);
+        rv[0] = bf_lo(u.x), rv[1] = bf_hi(u.x), rv[2] = bf_lo(u.y), rv[3] = bf_hi(u.y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < w.left) rv[i] = bf2f(rp[i]);
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int i = 0; i < nk; ++i) {
-        const int s = i % p.stages;
-        if (!mbar_wait(&sh.full[s], (i / p.stages) & 1, p.wait_ns)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t a = smem_u32(a_smem + s * A_BYTES), b = smem_u32(b_smem + s * p.b_bytes);
 #pragma unroll
-        for (int kk = 0; kk < KB / 32; ++kk)
-          umma_f8(tmem, sdesc_sw128(a + kk * 32), sdesc_sw128(b + kk * 32), p.idesc, (i | kk) != 0);
-        umma_commit(&sh.empty[s]);
-        issued = i + 1;
+    for (int i = 0; i < 4; ++i) {
+      o[i] = a4[i] * sx * w.sw[0][i];
+      if constexpr (SW) {
+        const float b4[4] = {acc[1].x, acc[1].y, acc[1].z, acc[1].w};
+        o[i] = silu(o[i]) * (b4[i] * sx * w.sw[1][i]);
       }
-      if (ok) {
-        umma_commit(&sh.done);
-      } else {
+      if constexpr (EPI == EPI_RESIDUAL) o[i] += rv[i];
+    }
+    bf16* op = p.out + (int64_t)m * p.ldo + w.j;
+    if (w.vec) {
+      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < w.left) op[i] = f2bf(o[i]);
+    }
+  };
+
+  // Warps 0 and 1 run their loops as whole warps with one elected lane issuing:
+  // ptxas keeps warp-uniform operands in uniform registers then (a loop inside
+  // one lane's branch costs 300 ns per block for the MMAs alone, this one
+  // 205 ns).  Ring position and phase are counted, not divided out of the block number.
+  if (warp == 0) {
+    if (elect_one()) {
+      prefetch_tmap(&amap);
+      prefetch_tmap(&bmap);
+      const int tile = tile_of(first_unit);
+      for (int i = 0; i < nk && i < p.stages; ++i) {
+        tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, SW ? tile * 64 : tile * TILE_J);
+        if (SW) tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, p.n_out + tile * 64);
+      }
+    }
+    __syncwarp();
+    pdl_wait();
+    const int bytes = A_BYTES + p.b_bytes;
+    int s = 0;
+    uint32_t phase = 1;   // a fresh barrier's previous phase counts as complete
+    bool ok = true;
+    for (int u = first_unit; ok && u < p.units; u += unit_step) {
+      // a stage's weight rows: 128 of one matrix, or 64 gate and 64 up rows
+      const int tile = tile_of(u), m0 = row_of(u);
+      const int row0 = SW ? tile * 64 : tile * TILE_J, row1 = p.n_out + tile * 64;
+      int x = k_lo * KB;
+      for (int i = 0; i < nk; ++i, x += KB) {
+        ok = warp_wait(&sh.empty[s], phase, p.wait_ns);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&sh.full[s], bytes);
+          uint8_t* a = a_smem + s * A_BYTES;
+          tma_load_2d(a, &amap, &sh.full[s], x, row0);
+          if (SW) tma_load_2d(a + A_BYTES / 2, &amap, &sh.full[s], x, row1);
+          tma_load_2d(b_smem + s * p.b_bytes, &bmap, &sh.full[s], x, m0);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(p.status, TSDS_E_TIMEOUT);
+      *(volatile int*)&sh.abort = 1;
+    }
+  } else if (warp == 1) {
+    bool ok = true;
+    const uint64_t a0 = sdesc_sw128(smem_u32(a_smem)), b0 = sdesc_sw128(smem_u32(b_smem));
+    int s = 0, buf = 0;
+    uint32_t phase = 0, tphase = 1;
+    for (int u = first_unit; ok && u < p.units; u += unit_step) {
+      ok = warp_wait(&sh.tempty[buf], tphase, p.wait_ns);
+      const uint32_t d = tmem + buf * p.tmem_cols;
+      if (ok && elect_one()) tc_fence_after();
+      for (int i = 0; ok && i < nk; ++i) {
+        ok = warp_wait(&sh.full[s], phase, p.wait_ns);
+        if (!ok) break;
+        if (elect_one()) {
+          tc_fence_after();
+          const uint64_t a = a0 + (uint32_t)(s * A_BYTES >> 4), b = b0 + (uint32_t)(s * p.b_bytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < KB / 32; ++kk) umma_f8(d, a + kk * 2, b + kk * 2, p.idesc, (i | kk) != 0);
+          umma_commit(&sh.empty[s]);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok && elect_one()) umma_commit(&sh.tfull[buf]);
+      __syncwarp();
+      if (++buf == p.bufs) {
+        buf = 0;
+        tphase ^= 1;
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicExch(p.status, TSDS_E_TIMEOUT);
+      *(volatile int*)&sh.abort = 1;
+    }
+  } else if (p.C == 1) {
+    // ---- epilogue of whole units: 16 token rows at a time through a small
+    // double-buffered staging area, so that stores are whole lines ----
+    pdl_wait();
+    const int quarter = warp & 3;   // the TMEM lanes this warp may read
+    const int et = threadIdx.x - 64, g4 = et % G * 4;
+    constexpr int STEP = 128 / G;
+    float* stg = reinterpret_cast<float*>(smem + p.out_off);
+    int buf = 0;
+    uint32_t tphase = 0;
+    for (int u = first_unit; u < p.units; u += unit_step) {
+      const Out w = out_of(tile_of(u), g4);
+      const int m0 = row_of(u), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+      // the four warps go on together or not at all
+      const bool ok = mbar_wait(&sh.tfull[buf], tphase, p.wait_ns);
+      if (!ok) {
         atomicExch(p.status, TSDS_E_TIMEOUT);
         *(volatile int*)&sh.abort = 1;
       }
+      if (!epi_all(ok)) break;
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t at = tmem + buf * p.tmem_cols + ((uint32_t)(quarter * 32) << 16);
+      for (int c = 0; c < rows; c += 16) {
+        float v[16];
+        tmem_ld16(at + c, v);
+        float* to = stg + (c & 16) * TILE_J + quarter * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i * TILE_J] = v[i];
+        epi_bar();
+        const float* from = stg + (c & 16) * TILE_J + g4;
+        if (w.left > 0) {
+#pragma unroll
+          for (int i = 0; i < 16; i += STEP) {
+            const int mc = i + et / G;
+            if (c + mc < rows) {
+              float4 acc[2];
+              acc[0] = *reinterpret_cast<const float4*>(from + mc * TILE_J);
+              if constexpr (SW) acc[1] = *reinterpret_cast<const float4*>(from + mc * TILE_J + 64);
+              finish(w, m0 + c + mc, acc);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      epi_bar();   // the staging area is free for the next unit
+      if (lane == 0) mbar_arrive(&sh.tempty[buf]);
+      if (++buf == p.bufs) {
+        buf = 0;
+        tphase ^= 1;
+      }
     }
   }
-  pdl_wait();
-  __syncwarp();
-  // done completes when every MMA has, so the ring is free for the partials
-  if (!mbar_wait(&sh.done, 0, p.wait_ns)) {
-    if (lane == 0) atomicExch(p.status, TSDS_E_TIMEOUT);
-    *(volatile int*)&sh.abort = 1;
+  if (p.C > 1) {
+    pdl_wait();
+    __syncwarp();
+    // tfull completes when every MMA has, so the ring is free for the partials
+    if (!mbar_wait(&sh.tfull[0], 0, p.wait_ns)) {
+      if (lane == 0) atomicExch(p.status, TSDS_E_TIMEOUT);
+      *(volatile int*)&sh.abort = 1;
+    }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -194,128 +368,102 @@ __global__ void __launch_bounds__(THREADS)
     if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
     __syncthreads();
   }
-
-  float* part = reinterpret_cast<float*>(smem);
-  const uint32_t part_addr = smem_u32(part);
-  const int rows = p.M - m_base < MAX_ROWS ? p.M - m_base : MAX_ROWS;
-  constexpr int G = SW ? 16 : 32;   // groups of four output channels per token row
-  const int j_base = SW ? tile * 64 : tile * TILE_J;
-  const bool wide = (p.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 &&
-                    (EPI != EPI_RESIDUAL || ((p.res_ld % 4) == 0 && (reinterpret_cast<uintptr_t>(p.res) & 7) == 0));
-  // token rows in chunks that fit the ring: partials [chunk][128] fp32
-  for (int c0 = 0; c0 < rows; c0 += p.chunk) {
-    const int cn = rows - c0 < p.chunk ? rows - c0 : p.chunk;
-    if (alive && warp >= 2) {
-      const int quarter = warp & 3;   // the TMEM lanes this warp may read
-      const int r = quarter * 32 + lane;
-      for (int c = 0; c < cn; c += 16) {
-        float v[16];
-        tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c0 + c, v);
+  if (p.C > 1) {
+    // ---- epilogue of a split unit: token rows in chunks that fit the ring, partials [chunk][128] fp32 ----
+    float* part = reinterpret_cast<float*>(smem);
+    const int g4 = threadIdx.x % G * 4;
+    constexpr int STEP = THREADS / G;
+    const Out w = out_of(tile_of(first_unit), g4);
+    const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+    for (int c0 = 0; c0 < rows; c0 += p.chunk) {
+      const int cn = rows - c0 < p.chunk ? rows - c0 : p.chunk;
+      if (alive && warp >= 2) {
+        const int quarter = warp & 3;
+        float* mine = part + quarter * 32 + lane;
+        for (int c = 0; c < cn; c += 16) {
+          float v[16];
+          tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c0 + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c + i < cn) part[(c + i) * TILE_J + r] = v[i];
-      }
-    }
-    unit_barrier(p.C);
-    const int total = cn * G, lo = rank * total / p.C, hi = (rank + 1) * total / p.C;
-    for (int e = lo + (int)threadIdx.x; alive && e < hi; e += THREADS) {
-      const int mc = e / G, g = e - mc * G;
-      const int m = m_base + c0 + mc, j = j_base + g * 4;
-      const uint32_t at = part_addr + (uint32_t)(mc * TILE_J + g * 4) * 4;
-      float4 acc[2];
-#pragma unroll
-      for (int h = 0; h < (SW ? 2 : 1); ++h) {
-        if (p.C == 1) {
-          acc[h] = *reinterpret_cast<const float4*>(part + mc * TILE_J + g * 4 + h * 64);
-        } else {
-          float4 f[MAX_C];
-#pragma unroll
-          for (int q = 0; q < MAX_C; ++q)
-            if (q < p.C) f[q] = ld_peer(mapa_shared(at + h * 256, q));
-          acc[h] = f[0];
-#pragma unroll
-          for (int q = 1; q < MAX_C; ++q)
-            if (q < p.C) acc[h] = add4(acc[h], f[q]);
+          for (int i = 0; i < 16; ++i)
+            if (c + i < cn) mine[(c + i) * TILE_J] = v[i];
         }
       }
-      const float sx = p.sx[m];
-      float o[4];
-      const float a4[4] = {acc[0].x, acc[0].y, acc[0].z, acc[0].w};
-      const float b4[4] = {acc[1].x, acc[1].y, acc[1].z, acc[1].w};
-      const int left = p.n_out - j;   // channels of this group inside the output
-      if (left <= 0) continue;
-      const bool vec = wide && left >= 4;
-      float rv[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (EPI == EPI_RESIDUAL) {
-        const bf16* rp = p.res + (int64_t)m * p.res_ld + j;
-        if (vec) {
-          const uint2 u = *reinterpret_cast<const uint2*>(rp);
-          rv[0] = bf_lo(u.x), rv[1] = bf_hi(u.x), rv[2] = bf_lo(u.y), rv[3] = bf_hi(u.y);
-        } else {
+      cluster_barrier();
+      if (alive && w.left > 0) {
+        // this CTA's token rows, from every CTA's partials in rank order
+        const int hi = (rank + 1) * cn / p.C;
+        for (int mc = rank * cn / p.C + (int)threadIdx.x / G; mc < hi; mc += STEP) {
+          const uint32_t at = smem_u32(part + mc * TILE_J + g4);
+          float4 acc[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < left) rv[i] = bf2f(rp[i]);
+          for (int h = 0; h < (SW ? 2 : 1); ++h) {
+            float4 f[MAX_C];
+#pragma unroll
+            for (int q = 0; q < MAX_C; ++q)
+              if (q < p.C) f[q] = ld_peer(mapa_shared(at + h * 256, q));
+            acc[h] = f[0];
+#pragma unroll
+            for (int q = 1; q < MAX_C; ++q)
+              if (q < p.C) acc[h] = add4(acc[h], f[q]);
+          }
+          finish(w, m0 + c0 + mc, acc);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int jj = i < left ? j + i : j;
-        o[i] = a4[i] * sx * p.sw[jj];
-        if constexpr (SW) o[i] = silu(o[i]) * (b4[i] * sx * p.sw[p.n_out + jj]);
-        if constexpr (EPI == EPI_RESIDUAL) o[i] += rv[i];
-      }
-      bf16* op = p.out + (int64_t)m * p.ldo + j;
-      if (vec) {
-        *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < left) op[i] = f2bf(o[i]);
-      }
+      cluster_barrier();   // the peers are done with this CTA's partials
     }
-    unit_barrier(p.C);   // the peers are done with this CTA's partials
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(p.bufs * p.tmem_cols));
   }
 }
 
-// Clusters of C CTAs with `smem` bytes each that the device holds at once
-// (0 if the query fails); cached per (C, smem), the devices of one process
-// assumed alike.
-template <int EPI>
-int resident_clusters(int C, size_t smem) {
-  struct Entry {
-    int C;
-    size_t smem;
-    int n;
-  };
-  static Entry cache[64];
-  static int used = 0;
-  std::lock_guard<std::mutex> hold(tsds_host_cache_lock());
-  for (int i = 0; i < used; ++i)
-    if (cache[i].C == C && cache[i].smem == smem) return cache[i].n;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, f8_gemm_kernel<EPI>, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    n = 0;
+// One way to place a launch: CTAs per SM, cluster size, ring depth.
+struct Shape {
+  int C = 1, stages = 0;
+  bool persistent = false;
+  long long grid = 0;
+  double cost = 1e30;   // estimated time, in units of its own
+};
+
+// What bounds the kernel up to 256 token rows is how many bytes of weights are
+// in flight: an SM holds a few hundred open requests, and a DRAM access
+// takes about a microsecond, so the rate grows with (CTAs x stages x 16 KB) up to
+// about 16 MB.  A launch whose units are all resident at once takes time
+// in inverse proportion to that.  One that is not goes in rounds, and its last
+// round lasts at least as long as one unit on one SM.  Measured: q/k/v
+// (80 units) at 26 rows 13.1 us on one CTA per SM (C = 1, 10 MB in flight),
+// 12.3 on two (C = 3, 16 MB and more); O (40 units) at 208 rows 22.1 us on one
+// (C = 3, 9.8 MB), 23.8 on two (C = 6, 7.8 MB); gate/up (400 units) at 128 rows
+// 49.7 us on one persistent CTA per SM, 60.4 on two.
+Shape shape_of(long long units, int KT, int npad, int tmem_cols, int ctas) {
+  Shape h;
+  const int sms = tsds_tc_num_sms();
+  const long long places = (long long)sms * ctas;
+  h.persistent = units > places;
+  if (ctas * tmem_cols * (h.persistent ? 2 : 1) > 512) return h;
+  int budget = SMEM_SM / ctas - SMEM_SIDE;
+  if (budget > SMEM_CTA) budget = SMEM_CTA;
+  h.stages = (budget - 1024 - (h.persistent ? STAGING : 0)) / (A_BYTES + npad * KB);
+  if (h.stages > RING) h.stages = RING;
+  // K over as many CTAs as keep the whole launch resident, with a tenth of
+  // the places to spare: clusters do not fill a GPC's SMs exactly, and one
+  // that has to wait for a place doubles the time
+  while (h.C < MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9) ++h.C;
+  h.grid = h.persistent ? places : units * h.C;
+  double waste = 1.0;
+  if (h.persistent) {
+    const long long full = (units - 1) / places;   // rounds before the last
+    const double last = (double)(units - full * places) / sms;
+    waste = (full * ctas + (last > 1.0 ? last : 1.0)) * sms / units;
   }
-  if (used < 64) cache[used++] = {C, smem, n};
-  return n;
+  double flight = (double)h.grid * h.stages * A_BYTES;
+  if (flight > 16e6) flight = 16e6;
+  h.cost = waste / flight;
+  return h;
 }
 
 template <int EPI>
@@ -325,6 +473,7 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   if (st != TSDS_OK) return st;
   constexpr bool SW = EPI == EPI_SWIGLU;
   const int tiles = SW ? (p.n_out + 63) / 64 : (p.n_out + TILE_J - 1) / TILE_J;
+  TSDS_RETURN_IF((long long)tiles * ((p.M + MAX_ROWS - 1) / MAX_ROWS) > 0x3fffffffll, TSDS_E_UNSUPPORTED);
   p.KT = (K + KB - 1) / KB;
   p.blocks = (p.M + MAX_ROWS - 1) / MAX_ROWS;
   const int widest = p.M < MAX_ROWS ? p.M : MAX_ROWS;
@@ -332,33 +481,29 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   p.b_bytes = p.npad * KB;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.npad) p.tmem_cols *= 2;
-  // CTAs per SM: three while three accumulators fit in TMEM's 512 columns and
-  // three stages in a third of the shared memory
-  int ctas = p.npad <= 64 ? 3 : 2;
-  const int stage = A_BYTES + p.b_bytes;
-  p.stages = (SMEM_SM / ctas - SMEM_SIDE - 1024) / stage;
-  if (p.stages > RING) p.stages = RING;
-  const size_t smem = (size_t)p.stages * stage + 1024;
-  p.chunk = p.stages * stage / (TILE_J * 4) / 16 * 16;
-  if (p.chunk > p.npad) p.chunk = p.npad;
-  const long long units = (long long)tiles * p.blocks;
-  p.C = 1;
-  for (int c = MAX_C; c > 1; --c) {
-    if (p.KT < 2 * c || units * c > (long long)tsds_tc_num_sms() * ctas) continue;
-    if (resident_clusters<EPI>(c, smem) >= units) {
-      p.C = c;
-      break;
-    }
+  Shape best;
+  for (int ctas = 1; ctas <= 3; ++ctas) {
+    const Shape h = shape_of((long long)tiles * p.blocks, p.KT, p.npad, p.tmem_cols, ctas);
+    if (h.stages >= 2 && h.cost <= best.cost) best = h;
   }
-  TSDS_RETURN_IF(units * p.C > 0x7fffffffll, TSDS_E_UNSUPPORTED);
+  TSDS_RETURN_IF(best.stages < 2, TSDS_E_UNSUPPORTED);
+  p.units = tiles * p.blocks;
+  p.C = best.C;
+  p.bufs = best.persistent ? 2 : 1;
+  p.stages = best.stages;
+  const int ring = p.stages * (A_BYTES + p.b_bytes);
+  p.out_off = best.persistent ? ring : 0;
+  const size_t smem = (size_t)ring + (best.persistent ? STAGING : 0) + 1024;
+  p.chunk = ring / (TILE_J * 4) / 16 * 16;
+  if (p.chunk > p.npad) p.chunk = p.npad;
   p.idesc = (1u << 4) | ((uint32_t)(p.npad >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
   p.wait_ns = tsds_get_wait_limit_ns();
   CUtensorMap amap, bmap;
-  st = tsds_make_tmap_2d_u8(&amap, w, K, SW ? 2 * (uint64_t)p.n_out : p.n_out, K, KB, 64);
+  st = tsds_make_tmap_2d_u8(&amap, w, K, SW ? 2 * (uint64_t)p.n_out : p.n_out, K, KB, SW ? 64 : TILE_J);
   if (st != TSDS_OK) return st;
   st = tsds_make_tmap_2d_u8(&bmap, x, K, p.M, ldx, KB, p.npad);
   if (st != TSDS_OK) return st;
-  const dim3 grid((unsigned)(units * p.C));
+  const dim3 grid((unsigned)best.grid);
   if (p.C > 1)
     tsds_launch_cluster(f8_gemm_kernel<EPI>, grid, dim3(THREADS), smem, stream, p.C, amap, bmap, p);
   else
