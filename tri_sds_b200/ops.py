@@ -36,7 +36,8 @@ def _p(t):
 
 
 def _stream():
-    return _VP(torch.cuda.current_stream().cuda_stream)
+    # the handle alone: building a torch.cuda.Stream for it takes 3.4 us a call
+    return _VP(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _need(cond, msg):
@@ -46,16 +47,16 @@ def _need(cond, msg):
 
 def _bf16_cuda(*ts):
     for t in ts:
-        if t is not None:
-            _need(t.is_cuda and t.dtype == torch.bfloat16, "expected a bf16 CUDA tensor")
+        if t is not None and not (t.is_cuda and t.dtype == torch.bfloat16):
+            raise ValueError("expected a bf16 CUDA tensor")
 
 
 def _cuda(dtype, *ts):
     """Index / length tensors: on a CUDA device, of the kernel's integer type
     (a host pointer handed to a kernel would fault the device)."""
     for t in ts:
-        if t is not None:
-            _need(t.is_cuda and t.dtype == dtype, f"expected a {dtype} CUDA tensor")
+        if t is not None and not (t.is_cuda and t.dtype == dtype):
+            raise ValueError(f"expected a {dtype} CUDA tensor")
 
 
 class _Scratch:
@@ -410,29 +411,36 @@ def accept_greedy(draft: torch.Tensor, target: torch.Tensor, target_len: torch.T
 FP8 = torch.float8_e4m3fn
 
 
-def _on(device, name: str, *args) -> None:
-    """_lib.call on `device`'s current stream; the tensors need not be on the
-    current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
+def _on(dev: int, name: str, *args) -> None:
+    """_lib.call on the current stream of device `dev`, which need not be the current one."""
+    if dev < 0 or dev == torch.cuda.current_device():
         _lib.call(name, *args, _stream())
         return
-    with torch.cuda.device(device):
+    with torch.cuda.device(dev):
         _lib.call(name, *args, _stream())
 
 
-def _one_device(t, *ts):
-    """The device of all the tensors given."""
+def _one_device(t, *ts) -> int:
+    """The device index of all the tensors given."""
+    dev = t.get_device()
     for o in ts:
-        _need(o is None or o.device == t.device, "tensors on different devices")
-    return t.device
+        if o is not None and o.get_device() != dev:
+            raise ValueError("tensors on different devices")
+    return dev
 
 
-def _rows(t, n: int, what: str):
-    """A 2-D row buffer of `n` columns with unit inner stride: its row stride
-    (of one row: n, whatever torch keeps there)."""
-    _need(t.dim() == 2 and t.shape[1] == n and (n == 1 or t.stride(1) == 1),
-          f"{what} must be [rows, {n}] with unit inner stride")
-    return t.stride(0) if t.shape[0] > 1 else n
+def _ld(t, rows: int, n: int, what: str) -> int:
+    """The row stride of a [rows, n] buffer with unit inner stride (of one
+    row: n, whatever torch keeps there)."""
+    st = t.stride()
+    if t.shape != (rows, n) or (st[1] != 1 and n > 1):
+        raise ValueError(f"{what} must be [{rows}, {n}] with unit inner stride")
+    return st[0] if rows > 1 else n
+
+
+def _vec(t, n: int, what: str) -> None:
+    if t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous [{n}]")
 
 
 def quant_fp8(x: torch.Tensor, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
@@ -440,15 +448,17 @@ def quant_fp8(x: torch.Tensor, out: torch.Tensor | None = None, scale: torch.Ten
     [rows] fp32) with scale = max|x| / 448 of the row, q = e4m3(x / scale).
     Weights ([out, in]: a scale per output channel) as well as activations."""
     _bf16_cuda(x)
-    _cuda(FP8, out)
-    _cuda(torch.float32, scale)
     _need(x.dim() == 2, "x must be [rows, n]")
     rows, n = x.shape
-    out = torch.empty(rows, n, dtype=FP8, device=x.device) if out is None else out
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device) if scale is None else scale
-    dev = _one_device(x, out, scale)
-    _need(out.shape[0] == rows and scale.shape == (rows,) and scale.is_contiguous(), "out / scale mismatch")
-    _on(dev, "tsds_quant_fp8", _p(x), _p(out), _p(scale), rows, n, _rows(x, n, "x"), _rows(out, n, "out"))
+    if out is None:
+        out = torch.empty(rows, n, dtype=FP8, device=x.device)
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _cuda(FP8, out)
+    _cuda(torch.float32, scale)
+    _vec(scale, rows, "scale")
+    _on(_one_device(x, out, scale), "tsds_quant_fp8", _p(x), _p(out), _p(scale), rows, n, _ld(x, rows, n, "x"),
+        _ld(out, rows, n, "out"))
     return out, scale
 
 
@@ -461,24 +471,29 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     Without a residual r = x and res_out is None.  norm_out, when given,
     receives y in bf16 (what per-request adapters read, see lora_add)."""
     _bf16_cuda(x, weight, residual, res_out, norm_out)
-    _cuda(FP8, out)
-    _cuda(torch.float32, scale)
     _need(x.dim() == 2, "x must be [rows, n]")
     rows, n = x.shape
-    _need(weight.shape == (n,) and weight.is_contiguous(), "weight must be [n]")
-    _need(residual is not None or res_out is None, "res_out without a residual")
-    out = torch.empty(rows, n, dtype=FP8, device=x.device) if out is None else out
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device) if scale is None else scale
-    if residual is not None and res_out is None:
-        res_out = torch.empty(rows, n, dtype=x.dtype, device=x.device)
-    dev = _one_device(x, weight, residual, out, scale, res_out, norm_out)
-    for t in (residual, out, res_out, norm_out):
-        _need(t is None or t.shape == (rows, n), "shape mismatch")
-    _need(scale.shape == (rows,) and scale.is_contiguous(), "scale must be [rows]")
-    ld_res, ld_out = (n, n) if residual is None else (_rows(residual, n, "residual"), _rows(res_out, n, "res_out"))
-    _on(dev, "tsds_add_rms_norm_fp8", _p(x), _p(residual), _p(weight), _p(res_out), _p(out), _p(scale), _p(norm_out),
-        rows, n, _rows(x, n, "x"), ld_res, ld_out, _rows(out, n, "out"),
-        n if norm_out is None else _rows(norm_out, n, "norm_out"), float(eps))
+    dev = x.device
+    if out is None:
+        out = torch.empty(rows, n, dtype=FP8, device=dev)
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    _cuda(FP8, out)
+    _cuda(torch.float32, scale)
+    _vec(weight, n, "weight")
+    _vec(scale, rows, "scale")
+    ld_res = ld_out = ld_norm = n
+    if residual is None:
+        _need(res_out is None, "res_out without a residual")
+    else:
+        if res_out is None:
+            res_out = torch.empty(rows, n, dtype=torch.bfloat16, device=dev)
+        ld_res, ld_out = _ld(residual, rows, n, "residual"), _ld(res_out, rows, n, "res_out")
+    if norm_out is not None:
+        ld_norm = _ld(norm_out, rows, n, "norm_out")
+    _on(_one_device(x, weight, residual, out, scale, res_out, norm_out), "tsds_add_rms_norm_fp8", _p(x), _p(residual),
+        _p(weight), _p(res_out), _p(out), _p(scale), _p(norm_out), rows, n, _ld(x, rows, n, "x"), ld_res, ld_out,
+        _ld(out, rows, n, "out"), ld_norm, float(eps))
     return out, scale, res_out
 
 
@@ -486,14 +501,16 @@ def _fp8_operands(x, x_scale, w, w_scale, n_out, out):
     """Checks of the 8-bit projections; returns (M, K, out)."""
     _cuda(FP8, x, w)
     _cuda(torch.float32, x_scale, w_scale)
-    _bf16_cuda(out)
-    _need(x.dim() == 2 and w.dim() == 2, "x must be [M, K] and w [out, K]")
+    _need(x.dim() == 2, "x must be [M, K]")
     M, K = x.shape
-    _need(w.shape[1] == K and w.is_contiguous(), "w must be contiguous [out, K]")
-    _need(x_scale.shape == (M,) and x_scale.is_contiguous(), "x_scale must be [M]")
-    _need(w_scale.shape == (w.shape[0],) and w_scale.is_contiguous(), "w_scale must hold a scale per row of w")
-    out = torch.empty(M, n_out, dtype=torch.bfloat16, device=x.device) if out is None else out
-    _need(out.shape == (M, n_out), "out must be [M, out]")
+    if w.shape[1] != K or not w.is_contiguous():
+        raise ValueError("w must be contiguous [out, K]")
+    _vec(x_scale, M, "x_scale")
+    _vec(w_scale, w.shape[0], "w_scale (a scale per row of w)")
+    if out is None:
+        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=x.device)
+    else:
+        _bf16_cuda(out)
     return M, K, out
 
 
@@ -501,24 +518,24 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
                out: torch.Tensor | None = None):
     """(x * x_scale) @ (w * w_scale)^T -> bf16 [M, n_out] for e4m3 x [M, K]
     (a scale per row) and w [n_out, K] (a scale per output channel)."""
+    _need(w.dim() == 2, "w must be [out, K]")
     n_out = w.shape[0]
     M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
-    dev = _one_device(x, x_scale, w, w_scale, out)
-    _on(dev, "tsds_linear_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(out),
-        _rows(out, n_out, "out"), M, n_out, K, _p(_scratch.status_word(dev)))
+    _on(_one_device(x, x_scale, w, w_scale, out), "tsds_linear_fp8", _p(x), _ld(x, M, K, "x"), _p(x_scale), _p(w),
+        _p(w_scale), _p(out), _ld(out, M, n_out, "out"), M, n_out, K, _p(_scratch.status_word(x.device)))
     return out
 
 
 def linear_residual_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                         res: torch.Tensor, out: torch.Tensor | None = None):
     """res + the 8-bit projection of linear_fp8, rounded once; out may be res."""
+    _need(w.dim() == 2, "w must be [out, K]")
     n_out = w.shape[0]
-    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
     _bf16_cuda(res)
-    _need(res.shape == (M, n_out), "res must be [M, n_out]")
-    dev = _one_device(x, x_scale, w, w_scale, out, res)
-    _on(dev, "tsds_linear_residual_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(res),
-        _rows(res, n_out, "res"), _p(out), _rows(out, n_out, "out"), M, n_out, K, _p(_scratch.status_word(dev)))
+    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
+    _on(_one_device(x, x_scale, w, w_scale, out, res), "tsds_linear_residual_fp8", _p(x), _ld(x, M, K, "x"),
+        _p(x_scale), _p(w), _p(w_scale), _p(res), _ld(res, M, n_out, "res"), _p(out), _ld(out, M, n_out, "out"), M,
+        n_out, K, _p(_scratch.status_word(x.device)))
     return out
 
 
@@ -526,12 +543,12 @@ def linear_swiglu_fp8(x: torch.Tensor, x_scale: torch.Tensor, w_gate_up: torch.T
                       out: torch.Tensor | None = None):
     """silu(gate) * up of the 8-bit projections for w_gate_up = [gate; up]
     ([2I, K] e4m3, 2I scales) -> bf16 [M, I], rounded once."""
-    _need(w_gate_up.shape[0] % 2 == 0, "w_gate_up must be [2I, K]")
+    _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] % 2 == 0, "w_gate_up must be [2I, K]")
     I = w_gate_up.shape[0] // 2
     M, K, out = _fp8_operands(x, x_scale, w_gate_up, w_scale, I, out)
-    dev = _one_device(x, x_scale, w_gate_up, w_scale, out)
-    _on(dev, "tsds_linear_swiglu_fp8", _p(x), _rows(x, K, "x"), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(out),
-        _rows(out, I, "out"), M, I, K, _p(_scratch.status_word(dev)))
+    _on(_one_device(x, x_scale, w_gate_up, w_scale, out), "tsds_linear_swiglu_fp8", _p(x), _ld(x, M, K, "x"),
+        _p(x_scale), _p(w_gate_up), _p(w_scale), _p(out), _ld(out, M, I, "out"), M, I, K,
+        _p(_scratch.status_word(x.device)))
     return out
 
 
@@ -550,18 +567,20 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     _cuda(torch.int32, adapter, ranks)
     _cuda(torch.float32, scale)
     _need(y.dim() == 2 and x.dim() == 2 and lora_a.dim() == 3 and lora_b.dim() == 3, "bad dimensions")
-    (M, N), K = y.shape, x.shape[1]
+    M, N = y.shape
+    K = x.shape[1]
     n_ad, R, S = lora_a.shape[0], lora_b.shape[2], 1 if slices is None else len(slices)
-    _need(x.shape[0] == M and lora_a.shape == (n_ad, S * R, K) and lora_b.shape == (n_ad, N, R), "shape mismatch")
+    if lora_a.shape != (n_ad, S * R, K) or lora_b.shape != (n_ad, N, R):
+        raise ValueError(f"lora_a must be [adapters, {S * R}, {K}] and lora_b [adapters, {N}, R]")
     _need(lora_a.is_contiguous() and lora_b.is_contiguous(), "lora_a and lora_b must be contiguous")
-    _need(adapter.shape == (M,) and adapter.is_contiguous(), "adapter must be [M]")
+    _vec(adapter, M, "adapter")
     for t in (scale, ranks):
-        _need(t is None or (t.shape == (n_ad,) and t.is_contiguous()), "scale and ranks hold a value per adapter")
-    out = torch.empty(M, N, dtype=y.dtype, device=y.device) if out is None else out
-    _need(out.shape == y.shape, "out must have y's shape")
-    dev = _one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out)
+        if t is not None:
+            _vec(t, n_ad, "scale and ranks (a value per adapter)")
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=y.device)
     widths = None if slices is None else (ctypes.c_int32 * S)(*slices)
-    _on(dev, "tsds_lora_add", _p(y), _rows(y, N, "y"), _p(x), _rows(x, K, "x"), _p(lora_a), _p(lora_b), _p(adapter),
-        _p(scale), _p(ranks), _p(out), _rows(out, N, "out"), M, K, N, n_ad, R, S, widths,
-        _p(_scratch.status_word(dev)))
+    _on(_one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out), "tsds_lora_add", _p(y), _ld(y, M, N, "y"), _p(x),
+        _ld(x, M, K, "x"), _p(lora_a), _p(lora_b), _p(adapter), _p(scale), _p(ranks), _p(out), _ld(out, M, N, "out"),
+        M, K, N, n_ad, R, S, widths, _p(_scratch.status_word(y.device)))
     return out
