@@ -274,7 +274,10 @@ int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const v
 int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, const void* lora_a, const void* lora_b,
                   const int32_t* adapter, const float* scale, const int32_t* ranks, void* out, int ldo,
                   int M, int K, int N, int n_adapters, int R, int n_slices, const int32_t* slice_widths,
-                  int32_t* status, tsds_stream_t stream);
+                  void* workspace, size_t workspace_bytes, int32_t* status, tsds_stream_t stream);
+/* 0 for a few rows; else the bytes that hold A x between the call's two
+ * launches (16-byte aligned, any contents). */
+size_t tsds_lora_workspace_bytes(int M, int R, int n_slices);
 
 /* ---------------------------------------------------------------------------
  * Verify / decode attention of T new tokens per sequence over the KV cache.

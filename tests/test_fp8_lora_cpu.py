@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-INVALID, ALIGN, UNSUPPORTED = 1, 2, 6
+INVALID, ALIGN, WORKSPACE, UNSUPPORTED = 1, 2, 4, 6
 BF, F32, I32, E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
 
 
@@ -68,10 +68,10 @@ def test_linear_codes(lib):
 
 def test_lora_codes(lib):
     def call(y=A, ldy=64, x=A, ldx=64, a=A, b=A, ad=A, out=A + 65536, ldo=64, M=2, K=64, N=64, n_ad=2, R=16, S=1,
-             widths=None, st=A):
+             widths=None, ws=A, wsb=1 << 30, st=A):
         w = None if widths is None else (ctypes.c_int32 * len(widths))(*widths)
         return lib.tsds_lora_add(P(y), ldy, P(x), ldx, P(a), P(b), P(ad), None, None, P(out), ldo, M, K, N, n_ad, R, S,
-                                 w, P(st), None)
+                                 w, P(ws), wsb, P(st), None)
     assert call(M=0) == 0
     for bad in (dict(M=-1), dict(K=0), dict(K=60), dict(N=0), dict(N=60), dict(n_ad=0), dict(R=0), dict(R=12),
                 dict(ldx=56), dict(ldy=56), dict(ldo=56), dict(S=0), dict(S=2), dict(S=2, widths=[32, 16]),
@@ -79,10 +79,13 @@ def test_lora_codes(lib):
                 dict(S=3, widths=[32, 32, 0]), dict(y=None), dict(x=None), dict(a=None), dict(b=None), dict(ad=None),
                 dict(out=None), dict(st=None), dict(out=A, ldo=72)):
         assert call(**bad) == INVALID, bad
+    for bad in (dict(M=1000, ws=None), dict(M=1000, wsb=64)):
+        assert call(**bad) == WORKSPACE, bad
+    assert lib.tsds_lora_workspace_bytes(8, 16, 3) == 0 and lib.tsds_lora_workspace_bytes(1000, 16, 3) > 0
     for bad in (dict(R=136), dict(S=5, widths=[32] * 5, N=160, ldy=160, ldo=160)):
         assert call(**bad) == UNSUPPORTED, bad
     for bad in (dict(y=A + 8), dict(x=A + 2), dict(a=A + 8), dict(b=A + 4), dict(out=A + 8), dict(ldx=68),
-                dict(ldy=68), dict(ldo=68)):
+                dict(ldy=68), dict(ldo=68), dict(M=1000, ws=A + 8)):
         assert call(**bad) == ALIGN, bad
 
 

@@ -46,7 +46,8 @@ def _check(ops, st, out=None):
     (1, 8, [8], 8, 1), (1, 5120, [1024, 128, 128], 16, 2), (8, 5120, [8192, 1024, 1024], 16, 8), (3, 40, [200], 24, 4),
     (16, 264, [32, 64, 96, 32], 128, 2), (17, 1000, [1000], 48, 3), (26, 2560, [2560], 64, 1), (100, 512, [96, 32], 8, 16),
     (208, 25600, [5120], 64, 8), (1024, 128, [256], 16, 5), (1025, 136, [264], 24, 5), (1500, 640, [640, 128, 128], 32, 4),
-    (2100, 72, [96, 96], 128, 3)])
+    (2100, 72, [96, 96], 128, 3), (40, 264, [32, 64, 96, 32], 128, 2), (130, 1000, [1000], 128, 3),
+    (257, 8, [8], 8, 2), (300, 1032, [2560], 64, 20), (520, 5120, [1024, 128, 128], 16, 70), (64, 640, [136], 128, 100)])
 @pytest.mark.parametrize("order", ["runs", "scattered"])
 def test_lora(ops, M, K, slices, R, n_ad, order):
     if order == "runs":      # requests of 5 rows each, every (n_ad + 1)-th without an adapter
@@ -71,10 +72,11 @@ def test_lora_without_scale_and_ranks(ops):
     _check(ops, _case(19, 512, [512], 32, 4, [m % 4 for m in range(19)], scale=False, ranks=False))
 
 
-def test_lora_unused_ranks_are_not_read_into_the_sum(ops):
+@pytest.mark.parametrize("M", [21, 300])
+def test_lora_unused_ranks_are_not_read_into_the_sum(ops, M):
     """NaN past an adapter's rank (in A's rows and in B's columns) changes nothing."""
-    for R, used in [(16, 1), (24, 7), (64, 33), (32, 0), (128, 66)]:
-        st = _case(21, 264, [96, 160], R, 2, [m % 2 for m in range(21)])
+    for R, used in [(16, 1), (24, 7), (64, 33), (32, 0), (128, 66), (72, 64), (104, 97)]:
+        st = _case(M, 264, [96, 160], R, 2, [m % 2 for m in range(M)])
         st["ranks"] = torch.tensor([used, R], dtype=torch.int32, device=DEV)
         for s in range(2):
             st["lora_a"][0, s * R + used:(s + 1) * R] = float("nan")
@@ -103,24 +105,26 @@ def test_lora_index_past_the_last_adapter_is_reported(ops, M):
     ref.check_bf16(got, want, err)
 
 
-def test_lora_strides_and_neighbours(ops):
+@pytest.mark.parametrize("M", [30, 390])
+def test_lora_strides_and_neighbours(ops, M):
     g = torch.Generator(device=DEV).manual_seed(2)
-    st = _case(30, 256, [128, 64], 16, 3, [(m // 7) - 1 for m in range(30)])
-    wide_x = torch.randn(30, 400, device=DEV, generator=g).to(BF)
+    st = _case(M, 256, [128, 64], 16, 3, [(m // (M // 4)) - 1 for m in range(M)])
+    wide_x = torch.randn(M, 400, device=DEV, generator=g).to(BF)
     st["x"] = wide_x[:, 64:320]
-    wide_y = torch.randn(30, 256, device=DEV, generator=g).to(BF)
+    wide_y = torch.randn(M, 256, device=DEV, generator=g).to(BF)
     st["y"] = wide_y[:, 32:224]
-    buf = torch.full((32, 264), 5.0, device=DEV, dtype=BF)
-    _check(ops, st, out=buf[1:31, 8:200])
+    buf = torch.full((M + 2, 264), 5.0, device=DEV, dtype=BF)
+    _check(ops, st, out=buf[1:M + 1, 8:200])
     keep = torch.ones_like(buf, dtype=torch.bool)
-    keep[1:31, 8:200] = False
+    keep[1:M + 1, 8:200] = False
     assert (buf[keep] == 5).all()
-    with pytest.raises(RuntimeError, match="status 10"):   # rows 28 and 29 name adapter 3 of 3
+    with pytest.raises(RuntimeError, match="status 10"):   # the last rows name adapter 3 of 3
         ops.check_status()
 
 
-def test_lora_nothing_to_add(ops):
-    st = _case(40, 128, [128], 16, 2, [-1] * 40)
+@pytest.mark.parametrize("M", [40, 700])
+def test_lora_nothing_to_add(ops, M):
+    st = _case(M, 128, [128], 16, 2, [-1] * M)
     assert torch.equal(ops.lora_add(**st), st["y"])
     y = st["y"].clone()
     assert torch.equal(ops.lora_add(**dict(st, y=y, out=y)), st["y"])
@@ -128,8 +132,9 @@ def test_lora_nothing_to_add(ops):
     assert ops.lora_add(**e).shape == (0, 128)
 
 
-def test_lora_same_bits_every_time(ops):
-    st = _case(208, 5120, [1024], 64, 8, [m // 26 for m in range(208)])
+@pytest.mark.parametrize("M,R", [(208, 64), (1040, 32)])
+def test_lora_same_bits_every_time(ops, M, R):
+    st = _case(M, 5120, [1024], R, 8, [m // (M // 8) for m in range(M)])
     first = ops.lora_add(**st)
     for _ in range(20):
         assert torch.equal(first, ops.lora_add(**st))
@@ -149,3 +154,32 @@ def test_lora_offsets_past_32_bits(ops):
     scale[-1] = st["scale"][0]
     got = ops.lora_add(st["y"], st["x"], a, b, torch.full((6,), n_ad - 1, dtype=torch.int32, device=DEV), scale=scale)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M", [24, 600])
+def test_lora_streams_and_graphs_share_nothing(ops, M):
+    """Two captured calls replayed at once on two streams, on changing inputs, beside eager calls."""
+    sts = [_case(M, 640, [512, 128], 32, 4, [(m // 40) % 5 - 1 for m in range(M)], seed=i) for i in range(3)]
+    want = [ops.lora_add(**st).clone() for st in sts]
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        st = {k: v.clone() if torch.is_tensor(v) else v for k, v in sts[0].items()}
+        side = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = ops.lora_add(**st)
+        graphs.append((graph, st, out, side))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for k, (graph, st, out, side) in enumerate(graphs):
+            with torch.cuda.stream(side):
+                for name, v in sts[(i + k) % 3].items():
+                    if torch.is_tensor(v):
+                        st[name].copy_(v)
+                graph.replay()
+        eager = ops.lora_add(**sts[(i + 2) % 3])
+        torch.cuda.synchronize()
+        for k, (_, _, out, _) in enumerate(graphs):
+            assert torch.equal(out, want[(i + k) % 3])
+        assert torch.equal(eager, want[(i + 2) % 3])

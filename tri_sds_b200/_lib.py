@@ -80,7 +80,8 @@ SIGNATURES = {
     "tsds_linear_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
     "tsds_linear_residual_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P]),
     "tsds_linear_swiglu_fp8": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P]),
-    "tsds_lora_add": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "tsds_lora_add": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P, _P]),
+    "tsds_lora_workspace_bytes": (_Z, [_I, _I, _I]),
     "tsds_logits_topk": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P]),
     "tsds_tree_state_bytes": (_Z, [_I]),
     "tsds_tree_init": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),

@@ -74,30 +74,8 @@ __device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint
       "l"(a), "l"(b), "r"(idesc), "r"(accum));
 }
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-  return p != 0;
-}
-
-// a bounded wait of a whole warp, with one outcome for all its lanes
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, uint64_t limit_ns) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, phase, limit_ns));
-}
-
-__device__ __forceinline__ float4 ld_peer(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
-}
-
-__device__ __forceinline__ void cluster_barrier() {
-  __syncwarp();
-  cluster_sync_all();
 }
 
 // whether `ok` holds in all 128 threads of the epilogue warps

@@ -1,0 +1,92 @@
+// What the two forms of the per-request adapters (lora.cu, lora_tc.cu) share: the
+// call's arguments and the grouping of a tile's token rows by adapter.
+#pragma once
+
+#include "common.cuh"
+
+namespace tsds {
+namespace lora {
+
+constexpr int MAX_SLICES = 4;
+constexpr int MAX_RANK = 128;
+constexpr int MAX_TILE = 64;   // rows per tile, at most
+constexpr int NEAR = 64;       // adapters whose rank and scale every CTA reads
+
+struct LoraArgs {
+  const bf16 *x, *y, *a, *b;
+  bf16* out;
+  const int32_t *adapter, *ranks;
+  const float* scale;
+  int32_t* status;
+  int64_t ldx, ldy, ldo;
+  int M, K, N, R, S, n_adapters, slots, ld_t;
+  int first_col[MAX_SLICES + 1];   // columns where the slices begin, and N
+};
+
+struct Tile {
+  int32_t id[MAX_TILE];      // adapter of each row; -1: none; -2: past the last row
+  unsigned long long leads;  // rows that are the first of their adapter
+  // rank and scale of the first adapters, read beside the rows' indices rather than after them
+  int32_t rank[NEAR];
+  float scale[NEAR];
+};
+
+struct Adapter {
+  int id, ra;   // index, rank
+  float scale;
+};
+
+// The rows row0 .. row0 + rows - 1 by adapter (rows <= MAX_TILE, at least 128
+// threads).  Rows without an adapter are a group of their own where `copies`.
+// An index past the last adapter is never followed: the row keeps its
+// projection, and the status says so where `report`.
+__device__ __forceinline__ void group_rows(const LoraArgs& p, Tile& sh, int row0, int rows, bool report,
+                                           bool copies) {
+  const int tid = threadIdx.x;
+  if (tid == 0) sh.leads = 0;
+  if (tid >= 64 && tid < 64 + NEAR) {
+    const int a = tid - 64;
+    sh.rank[a] = p.ranks && a < p.n_adapters ? p.ranks[a] : p.R;
+    sh.scale[a] = p.scale && a < p.n_adapters ? p.scale[a] : 1.0f;
+  }
+  if (tid < MAX_TILE) {
+    const int m = row0 + tid;
+    int id = tid < rows && m < p.M ? p.adapter[m] : -2;
+    if (tid < rows && m < p.M && id < 0) id = -1;
+    if (id >= p.n_adapters) {
+      id = -1;
+      if (report) atomicExch(p.status, TSDS_E_INDEX);
+    }
+    sh.id[tid] = id;
+  }
+  __syncthreads();
+  if (tid < rows) {
+    const int id = sh.id[tid];
+    bool first = true;
+#pragma unroll 16
+    for (int j = 0; j < rows; ++j) first = first && !(j < tid && sh.id[j] == id);
+    if (first && (id >= 0 || (id == -1 && copies))) atomicOr(&sh.leads, 1ull << tid);
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ Adapter adapter_of(const LoraArgs& p, const Tile& sh, int id) {
+  Adapter ad;
+  ad.id = id;
+  if (id < NEAR) {
+    ad.ra = sh.rank[id];
+    ad.scale = sh.scale[id];
+  } else {
+    ad.ra = p.ranks ? p.ranks[id] : p.R;
+    ad.scale = p.scale ? p.scale[id] : 1.0f;
+  }
+  ad.ra = ad.ra < 0 ? 0 : (ad.ra > p.R ? p.R : ad.ra);
+  return ad;
+}
+
+}  // namespace lora
+}  // namespace tsds
+
+// The two-launch form (lora_tc.cu) and the bytes of the workspace that holds its t.
+size_t tsds_lora_tc_workspace_bytes(int M, int R, int S);
+int tsds_lora_tc(const tsds::lora::LoraArgs& args, void* workspace, cudaStream_t stream);

@@ -1,0 +1,593 @@
+// Low-rank adapters beside a shared projection, for many token rows, on the
+// tcgen05 tensor cores (sm_100a); the formula and the one-launch kernel for few
+// rows are in lora.cu.  Two launches:
+//
+// * shrink: t[m][u] = scale * sum_k A[u][k] x[m][k].  A cluster of 8 CTAs takes
+//   a block of token rows and one adapter of those that occur in it, a CTA 1/8
+//   of K.  Rank rows fill the MMA's M, token rows are its N; x and A stream
+//   through a TMA ring.  The partial sums meet over distributed shared memory
+//   (rank order: always the same bits), and t is stored as two bf16 words
+//   (hi + lo, 16 bits of it), so its rounding is far below the output's.
+// * expand: out = y + B t^T, one CTA per 128 output channels x 64 token rows
+//   x adapter, several CTAs per SM: its y is requested while shrink still runs,
+//   the products of both words of t go into one TMEM accumulator, and the
+//   epilogue stores whole lines.
+//
+// The bytes of x and y bound both (B and A come from L2 after their first
+// use); the MMAs are a few percent of the tensor cores' rate.
+// shrink lets its successor start only after its own dependency wait, so
+// everything before shrink is complete when expand begins, and expand may
+// read y, B and the indices before its wait; only t comes after it.
+#include "common.cuh"
+#include "linear.cuh"
+#include "lora.cuh"
+#include "tc_core.cuh"
+
+using namespace tsds;
+using namespace tsds::tc;
+using namespace tsds::lora;
+
+namespace {
+
+constexpr int CL = 8;               // CTAs per shrink cluster
+constexpr int THREADS = 192;        // TMA warp, MMA warp, four epilogue warps
+constexpr int BKE = 64;             // elements of K (or ranks) per block: a 128-byte swizzle row
+constexpr int RING = 8;             // most stages
+constexpr int A_SLACK = TILE_J * 128;   // the MMA reads 128 rows of A, a stage may hold fewer
+
+struct ShrinkArgs {
+  LoraArgs l;
+  bf16* t;             // [M][2][ld_t]: hi, lo
+  int ld_t, Rp;        // columns of t; columns per slice
+  int nt, blocks;      // token rows per block, blocks
+  int arows, bx;       // rank rows per pass; rows of a small box
+  int KT, stages, stage_bytes;
+  uint32_t idesc;
+  int tmem_cols;
+  uint64_t wait_ns;
+};
+
+struct ShrinkShared {
+  Tile tile;
+  uint64_t full[RING], empty[RING], tfull, drain;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ void give_up(int32_t* status, int* abort, int lane) {
+  if (lane == 0) atomicExch(status, TSDS_E_TIMEOUT);
+  *(volatile int*)abort = 1;
+}
+
+__global__ void __launch_bounds__(THREADS)
+    shrink_kernel(const __grid_constant__ CUtensorMap a_all, const __grid_constant__ CUtensorMap a_box,
+                  const __grid_constant__ CUtensorMap xmap, ShrinkArgs p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ ShrinkShared sh;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  // every block's first adapter before any block's second: clusters without one come last
+  const int unit = blockIdx.x / CL, slot = unit / p.blocks, row0 = (unit - slot * p.blocks) * p.nt;
+  if (warp == 0 && elect_one()) {
+    prefetch_tmap(&a_all);
+    prefetch_tmap(&xmap);
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.tfull, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    fence_barrier_init();
+  }
+  pdl_wait();
+  pdl_trigger();   // after the wait: expand reads what comes before this kernel without one
+  group_rows(p.l, sh.tile, row0, p.nt, rank == 0 && slot == 0, false);
+  // a cluster whose turn never comes leaves before it takes TMEM
+  if (__popcll(sh.tile.leads) <= slot) return;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(p.tmem_cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  float* part = reinterpret_cast<float*>(smem);   // [nt][128], in the ring once it is free
+  const int k_lo = rank * p.KT / CL, nk = (rank + 1) * p.KT / CL - k_lo;
+  int s = 0, issued = 0;                 // ring position, blocks so far (warps 0 and 1)
+  uint32_t phase = warp == 0 ? 1 : 0, tphase = 0;
+  bool alive = true;
+
+  unsigned long long leads = sh.tile.leads;
+  for (int gi = 0; leads; ++gi, leads &= leads - 1) {
+    if (gi % p.l.slots != slot) continue;
+    const Adapter ad = adapter_of(p.l, sh.tile, sh.tile.id[__ffsll((long long)leads) - 1]);
+    const int ra16 = (ad.ra + 15) / 16 * 16;
+    for (int u0 = 0; ad.ra > 0 && u0 < p.l.S * p.l.R; u0 += p.arows) {   // rank rows u0 .. u0 + arows - 1
+      const bool all = ad.ra == p.l.R;
+      if (warp == 0 && alive) {
+        // small boxes of this pass: only the ranks that the adapter uses
+        int bytes = p.nt * 128 + p.arows * 128;
+        if (!all) {
+          bytes = p.nt * 128;
+          for (int u = u0; u < u0 + p.arows && u < p.l.S * p.l.R; u += p.bx)
+            if (u % p.l.R < ad.ra) bytes += p.bx * 128;
+        }
+        for (int i = 0; i < nk; ++i) {
+          alive = warp_wait(&sh.empty[s], phase, p.wait_ns);
+          if (!alive) break;
+          if (elect_one()) {
+            uint8_t* a = smem + s * p.stage_bytes;
+            const int k = (k_lo + i) * BKE, a_row = ad.id * p.l.S * p.l.R;
+            mbar_arrive_expect_tx(&sh.full[s], bytes);
+            tma_load_2d(a + p.arows * 128, &xmap, &sh.full[s], k, row0);
+            if (all) {
+              tma_load_2d(a, &a_all, &sh.full[s], k, a_row + u0);
+            } else {
+              for (int u = u0; u < u0 + p.arows && u < p.l.S * p.l.R; u += p.bx)
+                if (u % p.l.R < ad.ra) tma_load_2d(a + (u - u0) * 128, &a_box, &sh.full[s], k, a_row + u);
+            }
+          }
+          __syncwarp();
+          ++issued;
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (!alive) give_up(p.l.status, &sh.abort, lane);
+      } else if (warp == 1 && alive) {
+        for (int i = 0; i < nk; ++i) {
+          alive = warp_wait(&sh.full[s], phase, p.wait_ns);
+          if (!alive) break;
+          if (elect_one()) {
+            tc_fence_after();
+            const uint64_t a = sdesc_sw128(smem_u32(smem + s * p.stage_bytes));
+            const uint64_t b = sdesc_sw128(smem_u32(smem + s * p.stage_bytes + p.arows * 128));
+#pragma unroll
+            for (int kk = 0; kk < BKE / 16; ++kk) umma_bf16(tmem, a + kk * 2, b + kk * 2, p.idesc, (i | kk) != 0);
+            umma_commit(&sh.empty[s]);
+          }
+          __syncwarp();
+          ++issued;
+          if (++s == p.stages) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (alive && elect_one()) umma_commit(&sh.tfull);
+        __syncwarp();
+        if (!alive) give_up(p.l.status, &sh.abort, lane);
+      }
+      __syncwarp();
+      // a CTA without a block of K (K short of 8 blocks) has nothing to wait for
+      if (nk > 0) {
+        if (!mbar_wait(&sh.tfull, tphase, p.wait_ns)) give_up(p.l.status, &sh.abort, lane);
+        tphase ^= 1;
+      }
+      __syncwarp();
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      alive = !*(volatile int*)&sh.abort;
+      if (alive && warp >= 2) {
+        const int quarter = warp & 3;
+        float* mine = part + quarter * 32 + lane;
+        for (int c = 0; c < p.nt; c += 16) {
+          float v[16];
+          if (nk > 0) {
+            tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mine[(c + i) * TILE_J] = v[i];
+        }
+        tc_fence_before();
+      }
+      cluster_barrier();
+      // this CTA's token rows: four ranks at a time, from every CTA's partials
+      const int share = p.nt / CL, groups = p.l.S * (ra16 / 4);
+      for (int e = threadIdx.x; alive && e < share * groups; e += THREADS) {
+        const int i = rank * share + e / groups, gq = e % groups, sl = gq / (ra16 / 4), r = (gq - sl * (ra16 / 4)) * 4;
+        const int u = sl * p.l.R + r - u0;
+        // columns past the rank are zeros, written with the pass their slice begins in
+        const bool sum = r < ad.ra && u >= 0 && u < p.arows;
+        const int u_first = sl * p.l.R;
+        if (!sum && !(r >= ad.ra && u_first >= u0 && u_first < u0 + p.arows)) continue;
+        if (sh.tile.id[i] != ad.id) continue;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (sum) {
+          const uint32_t at = smem_u32(part + i * TILE_J + u);
+          float4 f[CL];
+#pragma unroll
+          for (int k = 0; k < CL; ++k) f[k] = ld_peer(mapa_shared(at, k));
+          float4 a = f[0];
+#pragma unroll
+          for (int k = 1; k < CL; ++k) a = make_float4(a.x + f[k].x, a.y + f[k].y, a.z + f[k].z, a.w + f[k].w);
+          const float w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = r + k < ad.ra ? w[k] * ad.scale : 0.f;
+        }
+        float h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = rbf(v[k]);
+        bf16* to = p.t + (int64_t)(row0 + i) * 2 * p.ld_t + sl * p.Rp + r;
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf2(h[0], h[1]), pack_bf2(h[2], h[3]));
+        *reinterpret_cast<uint2*>(to + p.ld_t) =
+            make_uint2(pack_bf2(v[0] - h[0], v[1] - h[1]), pack_bf2(v[2] - h[2], v[3] - h[3]));
+      }
+      // the peers are done with this CTA's partials; the ring may be loaded again
+      fence_proxy_async();
+      cluster_barrier();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (sh.abort) {
+    if (warp == 0 && lane == 0 && issued > 0) drain_tma_ring(sh.full, p.stages, issued);
+    if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+  }
+}
+
+constexpr int XN = 64;                      // token rows of an expand unit
+constexpr int X_THREADS = 320;              // TMA warp, MMA warp, two groups of four epilogue warps
+constexpr int B_TILE = TILE_J * 128;        // 128 channels x 64 ranks
+constexpr int T_TILE = XN * 128;            // 64 token rows x 64 ranks
+constexpr int X_STAGING = 2 * 16 * TILE_J * (int)sizeof(float);
+
+struct ExpandArgs {
+  LoraArgs l;
+  int ld_t, Rp, blocks, tiles, step, kb;    // step: CTAs that share a block's channel tiles; kb: blocks of 64 ranks
+  int first_tile[MAX_SLICES + 1];           // channel tiles where the slices begin
+  uint64_t wait_ns;
+};
+
+struct ExpandShared {
+  Tile tile;
+  uint64_t t_full, full[2], empty[2], tfull[2], tempty[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+
+// A channel tile: its slice, first channel, and the end of its slice.
+struct Channels {
+  int sl, lo, end;
+};
+__device__ __forceinline__ Channels channels_of(const ExpandArgs& p, int tile) {
+  Channels c;
+  c.sl = 0;
+#pragma unroll
+  for (int i = 1; i < MAX_SLICES; ++i)
+    if (i < p.l.S && tile >= p.first_tile[i]) c.sl = i;
+  c.lo = p.l.first_col[c.sl] + (tile - p.first_tile[c.sl]) * TILE_J;
+  c.end = p.l.first_col[c.sl + 1];
+  return c;
+}
+
+__device__ __forceinline__ void half_bar(int half) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+}
+
+__global__ void __launch_bounds__(X_THREADS, 2)
+    expand_kernel(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap tmap, ExpandArgs p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ ExpandShared sh;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // every block's first adapter before any block's second
+  const int per_slot = p.blocks * p.step, slot = blockIdx.x / per_slot, at_slot = blockIdx.x - slot * per_slot;
+  const int block = at_slot / p.step, tile0 = at_slot - block * p.step, row0 = block * XN;
+  if (warp == 0 && elect_one()) {
+    prefetch_tmap(&bmap);
+    prefetch_tmap(&tmap);
+    mbar_init(&sh.t_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.tfull[i], 1);
+      mbar_init(&sh.tempty[i], 8);   // one arrival per epilogue warp
+    }
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    fence_barrier_init();
+  }
+  pdl_trigger();
+  group_rows(p.l, sh.tile, row0, XN, false, p.l.out != p.l.y);
+  if (__popcll(sh.tile.leads) <= slot) {   // nothing for this CTA
+    pdl_wait();
+    return;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(2 * XN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int b_bytes = p.kb * B_TILE;
+  uint8_t *b_smem = smem, *t_smem = smem + 2 * b_bytes;   // t: [slice][kb][hi, lo]
+  float* stg = reinterpret_cast<float*>(t_smem + p.l.S * p.kb * 2 * T_TILE);
+  int buf = 0, issued = 0;     // ring position = accumulator: one B tile per output tile
+  uint32_t phase = 0;
+  bool ok = true, have_t = false;
+
+  unsigned long long leads = sh.tile.leads;
+  for (int gi = 0; leads && ok; ++gi, leads &= leads - 1) {
+    if (gi % p.l.slots != slot) continue;
+    const int id = sh.tile.id[__ffsll((long long)leads) - 1];
+    Adapter ad = {};
+    if (id >= 0) ad = adapter_of(p.l, sh.tile, id);
+    const int steps = (ad.ra + 15) / 16;   // of 16 ranks; 0: rows are copied
+    if (warp == 0) {
+      const int kb = (steps + 3) / 4;
+      for (int tile = tile0; steps > 0 && tile < p.tiles; tile += p.step) {
+        ok = warp_wait(&sh.empty[buf], phase ^ 1, p.wait_ns);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&sh.full[buf], kb * B_TILE);
+          for (int i = 0; i < kb; ++i)
+            tma_load_2d(b_smem + buf * b_bytes + i * B_TILE, &bmap, &sh.full[buf], i * BKE,
+                        id * p.l.N + channels_of(p, tile).lo);
+        }
+        __syncwarp();
+        if (!have_t) {   // every slice's t of these rows, once; the first read that waits for shrink
+          pdl_wait();
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&sh.t_full, p.l.S * p.kb * 2 * T_TILE);
+            for (int i = 0; i < p.l.S * p.kb; ++i) {
+              uint8_t* t = t_smem + i * 2 * T_TILE;
+              tma_load_2d(t, &tmap, &sh.t_full, i * BKE, row0);
+              tma_load_2d(t + T_TILE, &tmap, &sh.t_full, p.ld_t + i * BKE, row0);
+            }
+          }
+          __syncwarp();
+          have_t = true;
+        }
+        ++issued;
+        phase ^= buf;
+        buf ^= 1;
+      }
+    } else if (warp == 1) {
+      for (int tile = tile0; steps > 0 && tile < p.tiles; tile += p.step) {
+        ok = warp_wait(&sh.tempty[buf], phase ^ 1, p.wait_ns) && warp_wait(&sh.full[buf], phase, p.wait_ns) &&
+             warp_wait(&sh.t_full, 0, p.wait_ns);
+        if (!ok) break;
+        uint8_t* bs = b_smem + buf * b_bytes;
+        if (ad.ra & 15) {
+          // the last step's ranks past the adapter's: B's columns there are not
+          // part of it, whatever they hold
+          const int from = ad.ra & 63, to = ((ad.ra + 15) & ~15) - (ad.ra & ~63);
+          uint8_t* b = bs + (ad.ra / 64) * B_TILE;
+          for (int row = lane; row < TILE_J; row += 32)
+            for (int c = from; c < to; ++c)
+              *reinterpret_cast<uint16_t*>(b + row * 128 + (((c >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0;
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (elect_one()) {
+          tc_fence_after();
+          const uint32_t idesc =
+              (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XN >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
+          const uint64_t b0 = sdesc_sw128(smem_u32(bs));
+          const uint64_t t0 = sdesc_sw128(smem_u32(t_smem + channels_of(p, tile).sl * p.kb * 2 * T_TILE));
+          for (int i = 0; i < steps; ++i) {
+            const uint64_t b = b0 + (uint32_t)((i >> 2) * B_TILE >> 4) + (i & 3) * 2;
+            const uint64_t t = t0 + (uint32_t)((i >> 2) * 2 * T_TILE >> 4) + (i & 3) * 2;
+            umma_bf16(tmem + buf * XN, b, t + (T_TILE >> 4), idesc, i != 0);   // lo
+            umma_bf16(tmem + buf * XN, b, t, idesc, 1);                        // hi
+          }
+          umma_commit(&sh.empty[buf]);
+          umma_commit(&sh.tfull[buf]);
+        }
+        __syncwarp();
+        ++issued;
+        phase ^= buf;
+        buf ^= 1;
+      }
+    } else {
+      // two groups of 128 threads, 32 token rows each.  A thread's four channels
+      // of every fourth row: a warp's accesses are 256 contiguous bytes
+      const int half = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, g4 = (et & 31) * 4, tr = half * 32 + (et >> 5);
+      const int quarter = warp & 3;   // the TMEM lanes this warp may read
+      float* mine = stg + half * 16 * TILE_J;
+      bool rows[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rows[i] = sh.tile.id[tr + i * 4] == id;
+      auto load_y = [&](int tile, uint2 (&y)[8]) {
+        if (tile >= p.tiles) return;
+        const Channels c = channels_of(p, tile);
+        const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + c.lo + g4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c.lo + g4 < c.end && rows[i]) y[i] = *reinterpret_cast<const uint2*>(at + i * 4 * p.l.ldy);
+      };
+      auto finish = [&](int tile, const uint2 (&y)[8]) {
+        const Channels ch = channels_of(p, tile);
+        const bool in = ch.lo + g4 < ch.end;
+        if (steps > 0) {
+          // 128 threads go on together or not at all
+          if (!mbar_wait(&sh.tfull[buf], phase, p.wait_ns)) {
+            atomicExch(p.l.status, TSDS_E_TIMEOUT);
+            *(volatile int*)&sh.abort = 1;
+          }
+          __syncwarp();
+          half_bar(half);
+          ok = !*(volatile int*)&sh.abort;
+          half_bar(half);
+          if (!ok) return;
+          tc_fence_after();
+        }
+        bf16* to_out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + ch.lo + g4;
+#pragma unroll
+        for (int c = 0; c < 32; c += 16) {
+          if (steps > 0) {
+            float v[16];
+            tmem_ld16(tmem + buf * XN + ((uint32_t)(quarter * 32) << 16) + half * 32 + c, v);
+            float* to = mine + quarter * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) to[i * TILE_J] = v[i];
+            if (c == 16) {   // the accumulator is read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.tempty[buf]);
+            }
+            half_bar(half);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = c / 4 + i;
+            if (in && rows[k]) {
+              uint2 o = y[k];
+              if (steps > 0) {
+                const float4 d = *reinterpret_cast<const float4*>(mine + ((et >> 5) + i * 4) * TILE_J + g4);
+                o = make_uint2(pack_bf2(bf_lo(o.x) + d.x, bf_hi(o.x) + d.y), pack_bf2(bf_lo(o.y) + d.z, bf_hi(o.y) + d.w));
+              }
+              *reinterpret_cast<uint2*>(to_out + k * 4 * p.l.ldo) = o;
+            }
+          }
+          __syncwarp();
+          if (steps > 0) half_bar(half);   // the staging area is free
+        }
+        if (steps > 0) {
+          phase ^= buf;
+          buf ^= 1;
+        }
+      };
+      // the next tile's y is requested before this one's is used, in a register
+      // set of its own: loads are awaited by set, so one set would be awaited
+      // with the requests just made (5 us a tile instead of 1.2)
+      uint2 y0[8], y1[8];
+      load_y(tile0, y0);
+      if (steps == 0) pdl_wait();
+      for (int tile = tile0; ok && tile < p.tiles; tile += 2 * p.step) {
+        load_y(tile + p.step, y1);
+        finish(tile, y0);
+        if (!ok || tile + p.step >= p.tiles) break;
+        load_y(tile + 2 * p.step, y0);
+        finish(tile + p.step, y1);
+      }
+    }
+    if (warp < 2 && !ok) {
+      if (lane == 0) atomicExch(p.l.status, TSDS_E_TIMEOUT);
+      *(volatile int*)&sh.abort = 1;
+    }
+    __syncwarp();
+    __syncthreads();
+    ok = !*(volatile int*)&sh.abort;
+    __syncthreads();
+  }
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  if (sh.abort) {   // uniform: copies and MMAs in flight finish (bounded) before TMEM is freed
+    if (warp == 0 && lane == 0) {
+      drain_tma_ring(sh.full, 2, issued);
+      if (have_t) mbar_wait(&sh.t_full, 0, 20000000ull);
+    }
+    if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * XN));
+  }
+}
+
+int launch_shrink(const CUtensorMap& a_all, const CUtensorMap& a_box, const CUtensorMap& xmap, const ShrinkArgs& p,
+                  cudaStream_t stream) {
+  static tsds_device_flags limit_set;
+  const int st = tsds_smem_limit_once(shrink_kernel, 97 * 1024, limit_set);
+  if (st != TSDS_OK) return st;
+  const int smem = p.stages * p.stage_bytes + A_SLACK + 1024;
+  tsds_launch_cluster(shrink_kernel, dim3((unsigned)(p.blocks * p.l.slots * CL)), dim3(THREADS), smem, stream, CL,
+                      a_all, a_box, xmap, p);
+  return tsds_launch_status();
+}
+
+int rank_columns(int R) { return (R + BKE - 1) / BKE * BKE; }
+
+}  // namespace
+
+size_t tsds_lora_tc_workspace_bytes(int M, int R, int S) {
+  return (size_t)M * 2 * S * rank_columns(R) * sizeof(bf16);
+}
+
+int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
+  ShrinkArgs p = {};
+  p.l = l;
+  p.t = (bf16*)workspace;
+  p.Rp = rank_columns(l.R);
+  p.ld_t = l.S * p.Rp;
+  // token rows per shrink block: 32 for a few hundred rows (more clusters), 64 above
+  p.nt = l.M <= 512 ? 32 : 64;
+  p.blocks = (l.M + p.nt - 1) / p.nt;
+  const int SR = l.S * l.R;
+  p.arows = SR < TILE_J ? SR : TILE_J;
+  p.bx = l.R % 16 ? 8 : 16;
+  p.KT = (l.K + BKE - 1) / BKE;
+  p.stage_bytes = (p.arows + p.nt) * 128;
+  p.stages = (96 * 1024 - A_SLACK) / p.stage_bytes;
+  if (p.stages > RING) p.stages = RING;
+  p.tmem_cols = p.nt;
+  p.idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.nt >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
+  p.wait_ns = tsds_get_wait_limit_ns();
+  // A cluster (CTA) per adapter of a block of rows as long as all are resident at
+  // once; beyond that each takes several in turn.  One without an adapter
+  // holds the next launch up: with twice as many the q/k/v adapters of 2048
+  // rows take 61 us instead of 48.
+  auto slots_of = [&](int blocks, int rows, int most) {
+    int n = most / blocks;
+    n = n < 1 ? 1 : (n > rows ? rows : n);
+    return n > l.n_adapters + 1 ? l.n_adapters + 1 : n;
+  };
+  const int sms = tsds_tc_num_sms();
+  p.l.slots = slots_of(p.blocks, p.nt, 2 * sms / CL);
+  CUtensorMap a_all, a_box, xmap, bmap, tmap;
+  const uint64_t a_rows = (uint64_t)l.n_adapters * SR;
+  int st = tsds_make_tmap_2d_bf16(&a_all, l.a, l.K, a_rows, (uint64_t)l.K * 2, BKE, p.arows, 1);
+  if (st == TSDS_OK) st = tsds_make_tmap_2d_bf16(&a_box, l.a, l.K, a_rows, (uint64_t)l.K * 2, BKE, p.bx, 1);
+  if (st == TSDS_OK) st = tsds_make_tmap_2d_bf16(&xmap, l.x, l.K, l.M, (uint64_t)l.ldx * 2, BKE, p.nt, 1);
+  if (st == TSDS_OK)
+    st = tsds_make_tmap_2d_bf16(&bmap, l.b, l.R, (uint64_t)l.n_adapters * l.N, (uint64_t)l.R * 2, BKE, TILE_J, 1);
+  if (st == TSDS_OK)
+    st = tsds_make_tmap_2d_bf16(&tmap, workspace, 2 * (uint64_t)p.ld_t, l.M, 4 * (uint64_t)p.ld_t, BKE, XN, 1);
+  if (st != TSDS_OK) return st;
+
+  st = launch_shrink(a_all, a_box, xmap, p, stream);
+  if (st != TSDS_OK) return st;
+
+  ExpandArgs q = {};
+  q.l = l;
+  q.ld_t = p.ld_t;
+  q.Rp = p.Rp;
+  q.blocks = (l.M + XN - 1) / XN;
+  q.kb = p.Rp / BKE;
+  for (int i = 0; i < l.S; ++i)
+    q.first_tile[i + 1] = q.first_tile[i] + (l.first_col[i + 1] - l.first_col[i] + TILE_J - 1) / TILE_J;
+  q.tiles = q.first_tile[l.S];
+  q.wait_ns = p.wait_ns;
+  const int smem = 2 * q.kb * B_TILE + l.S * q.kb * 2 * T_TILE + X_STAGING + 1024;
+  // channel tiles of a block over as many CTAs as are resident at once
+  const int places = sms * (smem <= 112 * 1024 ? 2 : 1);
+  q.step = places / q.blocks;
+  q.step = q.step < 1 ? 1 : (q.step > q.tiles ? q.tiles : q.step);
+  q.l.slots = slots_of(q.blocks * q.step, XN, places);
+  static tsds_device_flags expand_set;
+  st = tsds_smem_limit_once(expand_kernel, 220 * 1024, expand_set);
+  if (st != TSDS_OK) return st;
+  tsds_launch(expand_kernel, dim3((unsigned)(q.blocks * q.step * q.l.slots)), dim3(X_THREADS), smem, stream, bmap, tmap,
+              q);
+  return tsds_launch_status();
+}

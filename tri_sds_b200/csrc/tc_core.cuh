@@ -55,6 +55,26 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 
 __device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// One lane of a fully active warp, known to the compiler as one: what it issues
+// keeps its operands in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// A bounded wait of a whole warp, with one outcome for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase, limit_ns));
+}
+
+// 16 bytes of another CTA's shared memory (addr: shared::cluster address).
+__device__ __forceinline__ float4 ld_peer(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
 // ---- stream-K bookkeeping ---------------------------------------------------
 // 32-bit arithmetic: W * P < 2^32 is checked on the host.
 __device__ __forceinline__ int it_begin(int p, int P, uint32_t W) { return (int)(((uint32_t)p * W) / (uint32_t)P); }
@@ -113,6 +133,12 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t saddr, uint32_t rank) {
 
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// the same for threads that may have diverged
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  cluster_sync_all();
 }
 
 __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,

@@ -580,7 +580,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     if out is None:
         out = torch.empty(M, N, dtype=torch.bfloat16, device=y.device)
     widths = None if slices is None else (ctypes.c_int32 * S)(*slices)
+    nb = _lib.query("tsds_lora_workspace_bytes", M, R, S)
+    # of this call alone: calls on several streams and captured graphs share nothing
+    ws = torch.empty(nb, dtype=torch.uint8, device=y.device) if nb else None
     _on(_one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out), "tsds_lora_add", _p(y), _ld(y, M, N, "y"), _p(x),
         _ld(x, M, K, "x"), _p(lora_a), _p(lora_b), _p(adapter), _p(scale), _p(ranks), _p(out), _ld(out, M, N, "out"),
-        M, K, N, n_ad, R, S, widths, _p(_scratch.status_word(y.device)))
+        M, K, N, n_ad, R, S, widths, _p(ws), nb, _p(_scratch.status_word(y.device)))
     return out
