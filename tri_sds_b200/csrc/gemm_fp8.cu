@@ -19,6 +19,11 @@
 //   accumulators in TMEM, so the epilogue of one unit runs under the main
 //   loop of the next and the ring never drains.
 //
+// Above 128 token rows a tile's X bytes outweigh its weights', and two CTAs
+// form a pair (tcgen05 cta_group::2): a unit is 256 weight rows, each CTA stages
+// its 128 of them and half of the token rows, one thread of the leader issues
+// the MMAs of both, and each CTA finishes the 128 rows in its own TMEM.
+//
 // Warp 0 requests the tiles (TMA, 128-byte swizzle), warp 1 issues
 // tcgen05.mma kind::f8f6f4 (fp32 accumulators in TMEM), warps 2-5 drain the
 // accumulators.  Before the dependency wait the first weight tiles are only
@@ -67,11 +72,32 @@ struct F8Shared {
   int abort;
 };
 
+template <int CG>
 __device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accum));
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum));
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+
+// Arrival on `bar` when every MMA issued so far is done: of this CTA, or (a
+// pair) of both CTAs of the pair whose cluster ranks `pair` has set.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t pair) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)pair)
+        : "memory");
+  else
+    umma_commit(bar);
 }
 
 __device__ __forceinline__ float4 add4(float4 a, float4 b) {
@@ -92,7 +118,7 @@ __device__ __forceinline__ bool epi_all(bool ok) {
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
-template <int EPI>
+template <int EPI, int CG>   // CG: CTAs per unit
 __global__ void __launch_bounds__(THREADS)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, F8Args p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -100,12 +126,15 @@ __global__ void __launch_bounds__(THREADS)
   __shared__ F8Shared sh;
   constexpr bool SW = EPI == EPI_SWIGLU;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = p.C > 1 ? (int)cluster_ctarank() : 0;
-  const int first_unit = blockIdx.x / p.C, unit_step = gridDim.x / p.C;
+  const int crank = p.C * CG > 1 ? (int)cluster_ctarank() : 0;
+  const int half = crank % CG, rank = crank / CG;            // of the pair; of the K split
+  const int first_unit = blockIdx.x / (p.C * CG), unit_step = gridDim.x / (p.C * CG);
+  const uint32_t lead = crank - half, pair = 3u << lead;     // a pair's leader, and both its CTAs
+  constexpr int ROWS = SW ? 64 : TILE_J;                     // output channels per CTA of a unit
   const int k_lo = rank * p.KT / p.C, nk = (rank + 1) * p.KT / p.C - k_lo;
-  // unit -> weight tile and first token row; token blocks fastest, so that the
-  // units in flight share their weights through L2
-  auto tile_of = [&](int u) { return u / p.blocks; };
+  // unit -> this CTA's weight tile and first token row; token blocks fastest, so
+  // that the units in flight share their weights through L2
+  auto tile_of = [&](int u) { return u / p.blocks * CG + half; };
   auto row_of = [&](int u) { return (u - u / p.blocks * p.blocks) * MAX_ROWS; };
 
   if (threadIdx.x == 0) {
@@ -115,19 +144,26 @@ __global__ void __launch_bounds__(THREADS)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.tfull[i], 1);
-      mbar_init(&sh.tempty[i], 4);   // one arrival per epilogue warp
+      mbar_init(&sh.tempty[i], 4 * CG);   // one arrival per epilogue warp
     }
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(p.bufs * p.tmem_cols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                   "r"(p.bufs * p.tmem_cols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                   "r"(p.bufs * p.tmem_cols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();   // both CTAs' barriers and TMEM exist
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   uint8_t* a_smem = smem;
@@ -144,7 +180,7 @@ __global__ void __launch_bounds__(THREADS)
   };
   auto out_of = [&](int tile, int g4) {
     Out w;
-    w.j = (SW ? tile * 64 : tile * TILE_J) + g4;
+    w.j = tile * ROWS + g4;
     w.left = p.n_out - w.j;
     w.vec = w.left >= 4 && (p.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 &&
             (EPI != EPI_RESIDUAL || ((p.res_ld % 4) == 0 && (reinterpret_cast<uintptr_t>(p.res) & 7) == 0));
@@ -199,30 +235,37 @@ __global__ void __launch_bounds__(THREADS)
       prefetch_tmap(&bmap);
       const int tile = tile_of(first_unit);
       for (int i = 0; i < nk && i < p.stages; ++i) {
-        tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, SW ? tile * 64 : tile * TILE_J);
-        if (SW) tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, p.n_out + tile * 64);
+        tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, tile * ROWS);
+        if (SW) tma_prefetch_l2_2d(&amap, (k_lo + i) * KB, p.n_out + tile * ROWS);
       }
     }
     __syncwarp();
     pdl_wait();
-    const int bytes = A_BYTES + p.b_bytes;
+    const int bytes = CG * (A_BYTES + p.b_bytes);   // a pair's land on the leader's barrier
     int s = 0;
     uint32_t phase = 1;   // a fresh barrier's previous phase counts as complete
     bool ok = true;
     for (int u = first_unit; ok && u < p.units; u += unit_step) {
       // a stage's weight rows: 128 of one matrix, or 64 gate and 64 up rows
-      const int tile = tile_of(u), m0 = row_of(u);
-      const int row0 = SW ? tile * 64 : tile * TILE_J, row1 = p.n_out + tile * 64;
+      const int row0 = tile_of(u) * ROWS, row1 = p.n_out + row0;
+      const int m0 = row_of(u) + half * (p.npad / CG);   // of a pair, half of the token rows each
       int x = k_lo * KB;
       for (int i = 0; i < nk; ++i, x += KB) {
         ok = warp_wait(&sh.empty[s], phase, p.wait_ns);
         if (!ok) break;
         if (elect_one()) {
-          mbar_arrive_expect_tx(&sh.full[s], bytes);
+          if (half == 0) mbar_arrive_expect_tx(&sh.full[s], bytes);
           uint8_t* a = a_smem + s * A_BYTES;
-          tma_load_2d(a, &amap, &sh.full[s], x, row0);
-          if (SW) tma_load_2d(a + A_BYTES / 2, &amap, &sh.full[s], x, row1);
-          tma_load_2d(b_smem + s * p.b_bytes, &bmap, &sh.full[s], x, m0);
+          if constexpr (CG == 2) {
+            const uint32_t bar = mapa_shared(smem_u32(&sh.full[s]), lead);
+            tma_load_2d_pair(a, &amap, bar, x, row0);
+            if (SW) tma_load_2d_pair(a + A_BYTES / 2, &amap, bar, x, row1);
+            tma_load_2d_pair(b_smem + s * p.b_bytes, &bmap, bar, x, m0);
+          } else {
+            tma_load_2d(a, &amap, &sh.full[s], x, row0);
+            if (SW) tma_load_2d(a + A_BYTES / 2, &amap, &sh.full[s], x, row1);
+            tma_load_2d(b_smem + s * p.b_bytes, &bmap, &sh.full[s], x, m0);
+          }
         }
         __syncwarp();
         ++issued;
@@ -241,7 +284,7 @@ __global__ void __launch_bounds__(THREADS)
     const uint64_t a0 = sdesc_sw128(smem_u32(a_smem)), b0 = sdesc_sw128(smem_u32(b_smem));
     int s = 0, buf = 0;
     uint32_t phase = 0, tphase = 1;
-    for (int u = first_unit; ok && u < p.units; u += unit_step) {
+    for (int u = first_unit; half == 0 && ok && u < p.units; u += unit_step) {
       ok = warp_wait(&sh.tempty[buf], tphase, p.wait_ns);
       const uint32_t d = tmem + buf * p.tmem_cols;
       if (ok && elect_one()) tc_fence_after();
@@ -252,8 +295,8 @@ __global__ void __launch_bounds__(THREADS)
           tc_fence_after();
           const uint64_t a = a0 + (uint32_t)(s * A_BYTES >> 4), b = b0 + (uint32_t)(s * p.b_bytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < KB / 32; ++kk) umma_f8(d, a + kk * 2, b + kk * 2, p.idesc, (i | kk) != 0);
-          umma_commit(&sh.empty[s]);
+          for (int kk = 0; kk < KB / 32; ++kk) umma_f8<CG>(d, a + kk * 2, b + kk * 2, p.idesc, (i | kk) != 0);
+          commit<CG>(&sh.empty[s], pair);
         }
         __syncwarp();
         ++issued;
@@ -262,7 +305,7 @@ __global__ void __launch_bounds__(THREADS)
           phase ^= 1;
         }
       }
-      if (ok && elect_one()) umma_commit(&sh.tfull[buf]);
+      if (ok && elect_one()) commit<CG>(&sh.tfull[buf], pair);
       __syncwarp();
       if (++buf == p.bufs) {
         buf = 0;
@@ -320,7 +363,12 @@ __global__ void __launch_bounds__(THREADS)
       }
       tc_fence_before();
       epi_bar();   // the staging area is free for the next unit
-      if (lane == 0) mbar_arrive(&sh.tempty[buf]);
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          mbar_arrive_remote(mapa_shared(smem_u32(&sh.tempty[buf]), lead));   // the leader's MMAs reuse it
+        else
+          mbar_arrive(&sh.tempty[buf]);
+      }
       if (++buf == p.bufs) {
         buf = 0;
         tphase ^= 1;
@@ -342,8 +390,12 @@ __global__ void __launch_bounds__(THREADS)
   tc_fence_after();
   const bool alive = !*(volatile int*)&sh.abort;
   if (!alive) {  // uniform: copies and MMAs in flight finish (bounded) before TMEM is freed
-    if (warp == 0 && lane == 0) drain_tma_ring(sh.full, p.stages, issued);
-    if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
+    // (a pair's land on the leader's barriers; the other CTA leaves after it)
+    if (warp == 0 && lane == 0 && half == 0) drain_tma_ring(sh.full, p.stages, issued);
+    if (warp == 1 && lane == 0 && issued > 0) {
+      commit<CG>(&sh.drain, pair);
+      mbar_wait(&sh.drain, 0, 20000000ull);
+    }
     __syncthreads();
   }
   if (p.C > 1) {
@@ -378,7 +430,7 @@ __global__ void __launch_bounds__(THREADS)
             float4 f[MAX_C];
 #pragma unroll
             for (int q = 0; q < MAX_C; ++q)
-              if (q < p.C) f[q] = ld_peer(mapa_shared(at + h * 256, q));
+              if (q < p.C) f[q] = ld_peer(mapa_shared(at + h * 256, q * CG + half));
             acc[h] = f[0];
 #pragma unroll
             for (int q = 1; q < MAX_C; ++q)
@@ -392,16 +444,19 @@ __global__ void __launch_bounds__(THREADS)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_barrier();   // the pair is done with both TMEM halves and barriers
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(p.bufs * p.tmem_cols));
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.bufs * p.tmem_cols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.bufs * p.tmem_cols));
   }
 }
 
-// One way to place a launch: CTAs per SM, cluster size, ring depth.
+// One way to place a launch: CTAs per unit, CTAs per SM, K split, ring depth.
 struct Shape {
-  int C = 1, stages = 0;
+  int CG = 1, C = 1, stages = 0;
   bool persistent = false;
   long long grid = 0;
   double cost = 1e30;   // estimated time, in units of its own
@@ -417,76 +472,86 @@ struct Shape {
 // 12.3 on two (C = 3, 16 MB and more); O (40 units) at 208 rows 22.1 us on one
 // (C = 3, 9.8 MB), 23.8 on two (C = 6, 7.8 MB); gate/up (400 units) at 128 rows
 // 49.7 us on one persistent CTA per SM, 60.4 on two.
-Shape shape_of(long long units, int KT, int npad, int tmem_cols, int ctas) {
+Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas, int CG) {
   Shape h;
+  h.CG = CG;
   const int sms = tsds_tc_num_sms();
-  const long long places = (long long)sms * ctas;
+  const long long units = (long long)((tiles + CG - 1) / CG) * blocks;
+  const long long places = (long long)sms * ctas / CG;   // units resident at once
   h.persistent = units > places;
   if (ctas * tmem_cols * (h.persistent ? 2 : 1) > 512) return h;
   int budget = SMEM_SM / ctas - SMEM_SIDE;
   if (budget > SMEM_CTA) budget = SMEM_CTA;
-  h.stages = (budget - 1024 - (h.persistent ? STAGING : 0)) / (A_BYTES + npad * KB);
+  h.stages = (budget - 1024 - (h.persistent ? STAGING : 0)) / (A_BYTES + npad / CG * KB);
   if (h.stages > RING) h.stages = RING;
   // K over as many CTAs as keep the whole launch resident, with a tenth of
   // the places to spare: clusters do not fill a GPC's SMs exactly, and one
   // that has to wait for a place doubles the time
-  while (h.C < MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9) ++h.C;
-  h.grid = h.persistent ? places : units * h.C;
+  while ((h.C + 1) * CG <= MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9) ++h.C;
+  h.grid = h.persistent ? places : units * h.C;   // in units' CTAs, CG of them each
   double waste = 1.0;
   if (h.persistent) {
     const long long full = (units - 1) / places;   // rounds before the last
-    const double last = (double)(units - full * places) / sms;
-    waste = (full * ctas + (last > 1.0 ? last : 1.0)) * sms / units;
+    const double last = (double)(units - full * places) * CG / sms;
+    waste = (full * ctas + (last > 1.0 ? last : 1.0)) * sms / (units * CG);
   }
-  double flight = (double)h.grid * h.stages * A_BYTES;
+  double flight = (double)h.grid * CG * h.stages * A_BYTES;
   if (flight > 16e6) flight = 16e6;
   h.cost = waste / flight;
   return h;
 }
 
+template <int EPI, int CG>
+int launch(const CUtensorMap& amap, const CUtensorMap& bmap, const F8Args& p, unsigned grid, size_t smem,
+           cudaStream_t stream) {
+  static tsds_device_flags limit_set;
+  const int st = tsds_smem_limit_once(f8_gemm_kernel<EPI, CG>, SMEM_CTA, limit_set);
+  if (st != TSDS_OK) return st;
+  if (p.C * CG > 1)
+    tsds_launch_cluster(f8_gemm_kernel<EPI, CG>, dim3(grid), dim3(THREADS), smem, stream, p.C * CG, amap, bmap, p);
+  else
+    tsds_launch(f8_gemm_kernel<EPI, CG>, dim3(grid), dim3(THREADS), smem, stream, amap, bmap, p);
+  return tsds_launch_status();
+}
+
 template <int EPI>
 int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream_t stream) {
-  static tsds_device_flags limit_set;
-  int st = tsds_smem_limit_once(f8_gemm_kernel<EPI>, SMEM_CTA, limit_set);
-  if (st != TSDS_OK) return st;
   constexpr bool SW = EPI == EPI_SWIGLU;
   const int tiles = SW ? (p.n_out + 63) / 64 : (p.n_out + TILE_J - 1) / TILE_J;
-  TSDS_RETURN_IF((long long)tiles * ((p.M + MAX_ROWS - 1) / MAX_ROWS) > 0x3fffffffll, TSDS_E_UNSUPPORTED);
   p.KT = (K + KB - 1) / KB;
   p.blocks = (p.M + MAX_ROWS - 1) / MAX_ROWS;
+  TSDS_RETURN_IF((long long)tiles * p.blocks > 0x3fffffffll, TSDS_E_UNSUPPORTED);
   const int widest = p.M < MAX_ROWS ? p.M : MAX_ROWS;
   p.npad = (widest + 15) / 16 * 16;
-  p.b_bytes = p.npad * KB;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.npad) p.tmem_cols *= 2;
   Shape best;
-  for (int ctas = 1; ctas <= 3; ++ctas) {
-    const Shape h = shape_of((long long)tiles * p.blocks, p.KT, p.npad, p.tmem_cols, ctas);
-    if (h.stages >= 2 && h.cost <= best.cost) best = h;
-  }
+  for (int CG = 1; CG <= (p.npad > TILE_J ? 2 : 1); ++CG)
+    for (int ctas = 1; ctas <= 3; ++ctas) {
+      const Shape h = shape_of(tiles, p.blocks, p.KT, p.npad, p.tmem_cols, ctas, CG);
+      if (h.stages >= 2 && h.cost <= best.cost) best = h;
+    }
   TSDS_RETURN_IF(best.stages < 2, TSDS_E_UNSUPPORTED);
-  p.units = tiles * p.blocks;
+  p.units = (tiles + best.CG - 1) / best.CG * p.blocks;
   p.C = best.C;
   p.bufs = best.persistent ? 2 : 1;
   p.stages = best.stages;
+  p.b_bytes = p.npad / best.CG * KB;
   const int ring = p.stages * (A_BYTES + p.b_bytes);
   p.out_off = best.persistent ? ring : 0;
   const size_t smem = (size_t)ring + (best.persistent ? STAGING : 0) + 1024;
   p.chunk = ring / (TILE_J * 4) / 16 * 16;
   if (p.chunk > p.npad) p.chunk = p.npad;
-  p.idesc = (1u << 4) | ((uint32_t)(p.npad >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
+  p.idesc = (1u << 4) | ((uint32_t)(p.npad >> 3) << 17) | ((uint32_t)(TILE_J * best.CG >> 4) << 24);
   p.wait_ns = tsds_get_wait_limit_ns();
   CUtensorMap amap, bmap;
-  st = tsds_make_tmap_2d_u8(&amap, w, K, SW ? 2 * (uint64_t)p.n_out : p.n_out, K, KB, SW ? 64 : TILE_J);
+  int st = tsds_make_tmap_2d_u8(&amap, w, K, SW ? 2 * (uint64_t)p.n_out : p.n_out, K, KB, SW ? 64 : TILE_J);
   if (st != TSDS_OK) return st;
-  st = tsds_make_tmap_2d_u8(&bmap, x, K, p.M, ldx, KB, p.npad);
+  st = tsds_make_tmap_2d_u8(&bmap, x, K, p.M, ldx, KB, p.npad / best.CG);
   if (st != TSDS_OK) return st;
-  const dim3 grid((unsigned)best.grid);
-  if (p.C > 1)
-    tsds_launch_cluster(f8_gemm_kernel<EPI>, grid, dim3(THREADS), smem, stream, p.C, amap, bmap, p);
-  else
-    tsds_launch(f8_gemm_kernel<EPI>, grid, dim3(THREADS), smem, stream, amap, bmap, p);
-  return tsds_launch_status();
+  const unsigned grid = (unsigned)(best.grid * best.CG);
+  return best.CG == 2 ? launch<EPI, 2>(amap, bmap, p, grid, smem, stream)
+                      : launch<EPI, 1>(amap, bmap, p, grid, smem, stream);
 }
 
 int check(const void* x, int ldx, const float* sx, const void* w, const float* sw, const void* out, int ldo, int M,
