@@ -79,13 +79,13 @@ def test_lora_codes(lib):
                 dict(S=3, widths=[32, 32, 0]), dict(y=None), dict(x=None), dict(a=None), dict(b=None), dict(ad=None),
                 dict(out=None), dict(st=None), dict(out=A, ldo=72)):
         assert call(**bad) == INVALID, bad
-    for bad in (dict(M=1000, ws=None), dict(M=1000, wsb=64)):
+    for bad in (dict(M=2000, ws=None), dict(M=2000, wsb=64)):
         assert call(**bad) == WORKSPACE, bad
-    assert lib.tsds_lora_workspace_bytes(8, 16, 3) == 0 and lib.tsds_lora_workspace_bytes(1000, 16, 3) > 0
+    assert lib.tsds_lora_workspace_bytes(8, 16, 3) == 0 and lib.tsds_lora_workspace_bytes(2000, 16, 3) > 0
     for bad in (dict(R=136), dict(S=5, widths=[32] * 5, N=160, ldy=160, ldo=160)):
         assert call(**bad) == UNSUPPORTED, bad
     for bad in (dict(y=A + 8), dict(x=A + 2), dict(a=A + 8), dict(b=A + 4), dict(out=A + 8), dict(ldx=68),
-                dict(ldy=68), dict(ldo=68), dict(M=1000, ws=A + 8)):
+                dict(ldy=68), dict(ldo=68), dict(M=2000, ws=A + 8)):
         assert call(**bad) == ALIGN, bad
 
 

@@ -47,7 +47,8 @@ def _check(ops, st, out=None):
     (16, 264, [32, 64, 96, 32], 128, 2), (17, 1000, [1000], 48, 3), (26, 2560, [2560], 64, 1), (100, 512, [96, 32], 8, 16),
     (208, 25600, [5120], 64, 8), (1024, 128, [256], 16, 5), (1025, 136, [264], 24, 5), (1500, 640, [640, 128, 128], 32, 4),
     (2100, 72, [96, 96], 128, 3), (40, 264, [32, 64, 96, 32], 128, 2), (130, 1000, [1000], 128, 3),
-    (257, 8, [8], 8, 2), (300, 1032, [2560], 64, 20), (520, 5120, [1024, 128, 128], 16, 70), (64, 640, [136], 128, 100)])
+    (257, 8, [8], 8, 2), (300, 1032, [2560], 64, 20), (520, 5120, [1024, 128, 128], 16, 70), (64, 640, [136], 128, 100), (1000, 264, [96, 32], 32, 3),
+    (512, 520, [512], 64, 4), (1030, 5120, [640, 128, 128], 64, 2)])
 @pytest.mark.parametrize("order", ["runs", "scattered"])
 def test_lora(ops, M, K, slices, R, n_ad, order):
     if order == "runs":      # requests of 5 rows each, every (n_ad + 1)-th without an adapter
@@ -72,7 +73,7 @@ def test_lora_without_scale_and_ranks(ops):
     _check(ops, _case(19, 512, [512], 32, 4, [m % 4 for m in range(19)], scale=False, ranks=False))
 
 
-@pytest.mark.parametrize("M", [21, 300])
+@pytest.mark.parametrize("M", [16, 21, 300, 1100])
 def test_lora_unused_ranks_are_not_read_into_the_sum(ops, M):
     """NaN past an adapter's rank (in A's rows and in B's columns) changes nothing."""
     for R, used in [(16, 1), (24, 7), (64, 33), (32, 0), (128, 66), (72, 64), (104, 97)]:
@@ -105,7 +106,7 @@ def test_lora_index_past_the_last_adapter_is_reported(ops, M):
     ref.check_bf16(got, want, err)
 
 
-@pytest.mark.parametrize("M", [30, 390])
+@pytest.mark.parametrize("M", [30, 390, 1302])
 def test_lora_strides_and_neighbours(ops, M):
     g = torch.Generator(device=DEV).manual_seed(2)
     st = _case(M, 256, [128, 64], 16, 3, [(m // (M // 4)) - 1 for m in range(M)])
@@ -156,7 +157,7 @@ def test_lora_offsets_past_32_bits(ops):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("M", [24, 600])
+@pytest.mark.parametrize("M", [12, 240, 1200])
 def test_lora_streams_and_graphs_share_nothing(ops, M):
     """Two captured calls replayed at once on two streams, on changing inputs, beside eager calls."""
     sts = [_case(M, 640, [512, 128], 32, 4, [(m // 40) % 5 - 1 for m in range(M)], seed=i) for i in range(3)]

@@ -36,10 +36,12 @@ using namespace tsds::lora;
 namespace {
 
 // Whether one launch of this file's kernel runs, or the two of lora_tc.cu: by
-// the size of t.  Measured (q/k/v of hidden 5120): 8 x 26 rows at rank 16 (t of
-// 10 K elements) 22 us here, 31 there; at rank 64 (40 K) 49 and 33; 2 x 256 rows
-// at rank 16 (25 K) 30 and 25; 2048 rows at rank 32 142 and 48.
-bool few_rows(int M, int R, int S) { return M <= 256 && (int64_t)M * S * R <= 16384; }
+// the rows, which this kernel takes 16 at a time, and the size of t.  Measured
+// (K 5120, outputs 10240 in three slices or 8192 -> 5120 in one): 512 rows at
+// rank 16 (t of 25 K elements) 17 us here, 25 there; 768 rows (37 K) 27 and 28;
+// 208 rows at rank 64 (40 K) 36 and 33; 1024 rows at rank 16 in one slice (16 K) 25
+// and 29, at rank 64 (66 K) 36 and 30; 2048 rows at rank 8 (16 K) 48 and 39.
+bool few_rows(int M, int R, int S) { return M <= 1024 && (int64_t)M * S * R <= 36864; }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -217,10 +219,11 @@ __device__ __forceinline__ void expand(const LoraArgs& p, const Tile& sh, const 
   }
 }
 
-// The first product.  NT: n8 rank tiles per pass over K, U: chunks of 32 k loaded together.
-template <int NT, int U, int WARPS>
+// The first product.  NT: n8 rank tiles per pass over K, U: chunks of 32 k loaded
+// together, PER_SM: CTAs per SM.
+template <int NT, int U, int WARPS, int PER_SM>
 struct First {
-  static constexpr int THREADS = WARPS * 32, PASS = NT, LDR = NT * 8 + 4;   // LDR: padded row of partial sums
+  static constexpr int CTAS = PER_SM, THREADS = WARPS * 32, PASS = NT, LDR = NT * 8 + 4;   // LDR: padded row of partial sums
   static constexpr int PART = WARPS * TR * LDR * (int)sizeof(float);   // the CTA's sum, behind those of its warps
   static constexpr int WORK = PART + TR * LDR * (int)sizeof(float);
 
@@ -293,7 +296,7 @@ struct First {
 };
 
 template <typename F>
-__global__ void __launch_bounds__(F::THREADS, 1) lora_kernel(LoraArgs p) {
+__global__ void __launch_bounds__(F::THREADS, F::CTAS) lora_kernel(LoraArgs p) {
   __shared__ Tile sh;
   extern __shared__ __align__(128) uint8_t dyn[];
   float* part = reinterpret_cast<float*>(dyn + F::PART);   // [TR][LDR] this CTA's sum, read by the cluster
@@ -421,6 +424,11 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
     TSDS_RETURN_IF(!tsds_aligned16(workspace), TSDS_E_ALIGN);
     return tsds_lora_tc(p, workspace, stream);
   }
-  if (n_slices * R <= 16) return launch_lora<First<2, 4, 16>>(p, stream);
-  return launch_lora<First<8, 2, 12>>(p, stream);
+  // One tile of rows is a matter of latency: many warps and loads per CTA (q/k/v
+  // adapters of 8 one-token requests 11.2 us, 14.2 with the smaller CTAs).  With
+  // several tiles two smaller CTAs per SM overlap (8 x 26 rows 14.5 us, 21.8 with
+  // the larger ones).
+  if (M > TR) return launch_lora<First<8, 1, 8, 2>>(p, stream);
+  if (n_slices * R <= 16) return launch_lora<First<2, 4, 16, 1>>(p, stream);
+  return launch_lora<First<8, 2, 12, 1>>(p, stream);
 }
