@@ -274,8 +274,18 @@ __device__ __forceinline__ Channels channels_of(const ExpandArgs& p, int tile) {
   return c;
 }
 
+// barrier of 128 epilogue threads; the second says whether `ok` holds in all of them
 __device__ __forceinline__ void half_bar(int half) {
   asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+}
+__device__ __forceinline__ bool half_all(int half, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(1 + half)
+      : "memory");
+  return r != 0;
 }
 
 __global__ void __launch_bounds__(X_THREADS, 2)
@@ -397,39 +407,47 @@ __global__ void __launch_bounds__(X_THREADS, 2)
         buf ^= 1;
       }
     } else {
-      // two groups of 128 threads, 32 token rows each.  A thread's four channels
-      // of every fourth row: a warp's accesses are 256 contiguous bytes
-      const int half = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, g4 = (et & 31) * 4, tr = half * 32 + (et >> 5);
+      // two groups of 128 threads, 32 token rows each.  A thread takes eight
+      // channels of every eighth row: 16 lanes access 256 contiguous bytes
+      const int half = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, g8 = (et & 15) * 8, tr = half * 32 + (et >> 4);
       const int quarter = warp & 3;   // the TMEM lanes this warp may read
       float* mine = stg + half * 16 * TILE_J;
-      bool rows[8];
+      bool rows[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rows[i] = sh.tile.id[tr + i * 4] == id;
-      auto load_y = [&](int tile, uint2 (&y)[8]) {
+      for (int i = 0; i < 4; ++i) rows[i] = sh.tile.id[tr + i * 8] == id;
+      auto load_y = [&](int tile, uint4 (&y)[4]) {
         if (tile >= p.tiles) return;
         const Channels c = channels_of(p, tile);
-        const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + c.lo + g4;
+        const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + c.lo + g8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c.lo + g4 < c.end && rows[i]) y[i] = *reinterpret_cast<const uint2*>(at + i * 4 * p.l.ldy);
+        for (int i = 0; i < 4; ++i)
+          if (c.lo + g8 < c.end && rows[i]) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
       };
-      auto finish = [&](int tile, const uint2 (&y)[8]) {
+      // a tile further ahead: its lines into L2, one per thread
+      const int pr = half * 32 + (et >> 2), pc = (et & 1) * 64;
+      const bool p_row = (et & 2) == 0 && sh.tile.id[pr] == id;
+      auto prefetch_y = [&](int tile) {
+        if (tile >= p.tiles || !p_row) return;
+        const Channels c = channels_of(p, tile);
+        if (c.lo + pc < c.end)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.l.y + (int64_t)(row0 + pr) * p.l.ldy + c.lo + pc));
+      };
+      auto finish = [&](int tile, const uint4 (&y)[4]) {
         const Channels ch = channels_of(p, tile);
-        const bool in = ch.lo + g4 < ch.end;
+        const bool in = ch.lo + g8 < ch.end;
         if (steps > 0) {
           // 128 threads go on together or not at all
-          if (!mbar_wait(&sh.tfull[buf], phase, p.wait_ns)) {
+          ok = mbar_wait(&sh.tfull[buf], phase, p.wait_ns);
+          if (!ok) {
             atomicExch(p.l.status, TSDS_E_TIMEOUT);
             *(volatile int*)&sh.abort = 1;
           }
           __syncwarp();
-          half_bar(half);
-          ok = !*(volatile int*)&sh.abort;
-          half_bar(half);
+          ok = half_all(half, ok);
           if (!ok) return;
           tc_fence_after();
         }
-        bf16* to_out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + ch.lo + g4;
+        bf16* to_out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + ch.lo + g8;
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {
           if (steps > 0) {
@@ -446,15 +464,17 @@ __global__ void __launch_bounds__(X_THREADS, 2)
             half_bar(half);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = c / 4 + i;
+          for (int i = 0; i < 2; ++i) {
+            const int k = c / 8 + i;
             if (in && rows[k]) {
-              uint2 o = y[k];
+              uint4 o = y[k];
               if (steps > 0) {
-                const float4 d = *reinterpret_cast<const float4*>(mine + ((et >> 5) + i * 4) * TILE_J + g4);
-                o = make_uint2(pack_bf2(bf_lo(o.x) + d.x, bf_hi(o.x) + d.y), pack_bf2(bf_lo(o.y) + d.z, bf_hi(o.y) + d.w));
+                const float4* d = reinterpret_cast<const float4*>(mine + ((et >> 4) + i * 8) * TILE_J + g8);
+                const float4 a = d[0], b = d[1];
+                o = make_uint4(pack_bf2(bf_lo(o.x) + a.x, bf_hi(o.x) + a.y), pack_bf2(bf_lo(o.y) + a.z, bf_hi(o.y) + a.w),
+                               pack_bf2(bf_lo(o.z) + b.x, bf_hi(o.z) + b.y), pack_bf2(bf_lo(o.w) + b.z, bf_hi(o.w) + b.w));
               }
-              *reinterpret_cast<uint2*>(to_out + k * 4 * p.l.ldo) = o;
+              *reinterpret_cast<uint4*>(to_out + k * 8 * p.l.ldo) = o;
             }
           }
           __syncwarp();
@@ -468,14 +488,18 @@ __global__ void __launch_bounds__(X_THREADS, 2)
       // the next tile's y is requested before this one's is used, in a register
       // set of its own: loads are awaited by set, so one set would be awaited
       // with the requests just made (5 us a tile instead of 1.2)
-      uint2 y0[8], y1[8];
+      uint4 y0[4], y1[4];
       load_y(tile0, y0);
+      prefetch_y(tile0 + p.step);
+      prefetch_y(tile0 + 2 * p.step);
       if (steps == 0) pdl_wait();
       for (int tile = tile0; ok && tile < p.tiles; tile += 2 * p.step) {
         load_y(tile + p.step, y1);
+        prefetch_y(tile + 3 * p.step);
         finish(tile, y0);
         if (!ok || tile + p.step >= p.tiles) break;
         load_y(tile + 2 * p.step, y0);
+        prefetch_y(tile + 4 * p.step);
         finish(tile + p.step, y1);
       }
     }
