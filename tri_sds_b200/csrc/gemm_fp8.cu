@@ -539,7 +539,12 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   p.b_bytes = p.npad / best.CG * KB;
   const int ring = p.stages * (A_BYTES + p.b_bytes);
   p.out_off = best.persistent ? ring : 0;
-  const size_t smem = (size_t)ring + (best.persistent ? STAGING : 0) + 1024;
+  size_t smem = (size_t)ring + (best.persistent ? STAGING : 0) + 1024;
+  // A CTA's part of the SM's shared memory is at least its part of TMEM's 512
+  // columns, so CTAs that fit an SM never wait for columns there: a cluster
+  // whose CTA waited for another stream's, and that one for this, would hang both.
+  const size_t least = (size_t)p.bufs * p.tmem_cols * SMEM_SM / 512 - SMEM_SIDE;
+  if (smem < least) smem = least < SMEM_CTA ? least : SMEM_CTA;
   p.chunk = ring / (TILE_J * 4) / 16 * 16;
   if (p.chunk > p.npad) p.chunk = p.npad;
   p.idesc = (1u << 4) | ((uint32_t)(p.npad >> 3) << 17) | ((uint32_t)(TILE_J * best.CG >> 4) << 24);

@@ -534,6 +534,8 @@ int launch_shrink(const CUtensorMap& a_all, const CUtensorMap& a_box, const CUte
   static tsds_device_flags limit_set;
   const int st = tsds_smem_limit_once(shrink_kernel, 97 * 1024, limit_set);
   if (st != TSDS_OK) return st;
+  // more of the SM's shared memory than of TMEM's columns (at least 57 KB for 64;
+  // expand: 65 KB for 128), so CTAs that fit an SM never wait for columns
   const int smem = p.stages * p.stage_bytes + A_SLACK + 1024;
   tsds_launch_cluster(shrink_kernel, dim3((unsigned)(p.blocks * p.l.slots * CL)), dim3(THREADS), smem, stream, CL,
                       a_all, a_box, xmap, p);
