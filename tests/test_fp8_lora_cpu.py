@@ -144,3 +144,83 @@ def test_shapes_and_types_are_checked(monkeypatch):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"case {i} was accepted")
+
+
+# -- torch.ops.tsds ------------------------------------------------------------------
+
+_STREAM = object()
+
+
+@pytest.fixture()
+def recorded(monkeypatch):
+    """Calls recorded instead of made; every pointer must reach the bytes its call's sizes say."""
+    import tri_sds_b200.torch_ops  # noqa: F401
+    from abi_extents import TRef
+    from tri_sds_b200 import _lib, ops as o
+
+    def dtype_only(dtype, *ts):
+        for t in ts:
+            o._need(t is None or t.dtype == dtype, f"expected {dtype}")
+    calls = []
+
+    def call(name, *a):
+        assert a[-1] is _STREAM, name
+        calls.append(name)
+        need = _extents(name, a[:-1])
+        assert need
+        for i, nbytes in need:
+            assert a[i] is None or a[i].bytes_left() >= nbytes, (name, i, nbytes)
+    monkeypatch.setattr(o, "_p", lambda t: None if t is None else TRef(t))
+    monkeypatch.setattr(o, "_stream", lambda: _STREAM)
+    monkeypatch.setattr(o, "_cuda", dtype_only)
+    monkeypatch.setattr(o, "_bf16_cuda", lambda *ts: dtype_only(BF, *ts))
+    monkeypatch.setattr(_lib, "call", call)
+    yield calls
+
+
+def _extents(name, a):
+    """[(argument, bytes it must reach)] from the meanings in include/tsds.h."""
+    def rows(m, ld, n, size):
+        return ((m - 1) * ld + n) * size
+    if name == "tsds_quant_fp8":
+        x, q, s, m, n, ldx, ldq = a
+        return [(0, rows(m, ldx, n, 2)), (1, rows(m, ldq, n, 1)), (2, m * 4)]
+    if name == "tsds_add_rms_norm_fp8":
+        m, n, ldx, ldr, ldo, ldq, ldn = a[7:14]
+        return [(0, rows(m, ldx, n, 2)), (1, rows(m, ldr, n, 2)), (2, n * 2), (3, rows(m, ldo, n, 2)),
+                (4, rows(m, ldq, n, 1)), (5, m * 4), (6, rows(m, ldn, n, 2))]
+    if name in ("tsds_linear_fp8", "tsds_linear_swiglu_fp8"):
+        x, ldx, sx, w, sw, out, ldo, m, n, k, st = a
+        wr = 2 * n if "swiglu" in name else n
+        return [(0, rows(m, ldx, k, 1)), (2, m * 4), (3, wr * k), (4, wr * 4), (5, rows(m, ldo, n, 2)), (10, 4)]
+    if name == "tsds_linear_residual_fp8":
+        x, ldx, sx, w, sw, res, ldr, out, ldo, m, n, k, st = a
+        return [(0, rows(m, ldx, k, 1)), (2, m * 4), (3, n * k), (4, n * 4), (5, rows(m, ldr, n, 2)),
+                (7, rows(m, ldo, n, 2)), (12, 4)]
+    if name == "tsds_lora_add":
+        y, ldy, x, ldx, la, lb, ad, sc, rk, out, ldo, m, k, n, na, r, s, wd, ws, nb, st = a
+        return [(0, rows(m, ldy, n, 2)), (2, rows(m, ldx, k, 2)), (4, na * s * r * k * 2), (5, na * n * r * 2),
+                (6, m * 4), (7, na * 4), (8, na * 4), (9, rows(m, ldo, n, 2)), (18, nb), (20, 4)]
+    return []
+
+
+def test_torch_ops_calls_and_extents(recorded):
+    import tri_sds_b200.torch_ops as T
+    tsds = torch.ops.tsds
+    for name in T.PROJECTION_OPS:
+        schema = getattr(tsds, name).default._schema
+        assert not any(a.alias_info is not None and a.alias_info.is_write for a in schema.arguments), name
+    x, w, q, s = torch.zeros(5, 64).to(BF), torch.zeros(64).to(BF), torch.zeros(5, 64).to(E4M3), torch.zeros(5)
+    wq, ws, y = torch.zeros(48, 64).to(E4M3), torch.zeros(48), torch.zeros(5, 48).to(BF)
+    assert [t.shape for t in tsds.quant_fp8(x)] == [(5, 64), (5,)]
+    assert [t.shape for t in tsds.add_rms_norm_fp8(x, x, w)] == [(5, 64), (5,), (5, 64), (5, 64)]
+    assert tsds.linear_fp8(q, s, wq, ws).shape == (5, 48)
+    assert tsds.linear_residual_fp8(q, s, wq, ws, y).shape == (5, 48)
+    assert tsds.linear_swiglu_fp8(q, s, wq, ws).shape == (5, 24)
+    for m in (5, 2000):   # one launch, and two with a workspace
+        a, b, ad = torch.zeros(3, 32, 64).to(BF), torch.zeros(3, 96, 16).to(BF), torch.zeros(m, dtype=I32)
+        out = tsds.lora_add(torch.zeros(m, 96).to(BF), torch.zeros(m, 64).to(BF), a, b, ad, torch.ones(3),
+                            torch.ones(3, dtype=I32), [64, 32])
+        assert out.shape == (m, 96)
+    assert recorded == ["tsds_quant_fp8", "tsds_add_rms_norm_fp8", "tsds_linear_fp8", "tsds_linear_residual_fp8",
+                        "tsds_linear_swiglu_fp8", "tsds_lora_add", "tsds_lora_add"]

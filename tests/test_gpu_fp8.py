@@ -351,3 +351,25 @@ def test_block_captured_and_replayed_on_a_side_stream(ops):
         for k, (_, _, _, out) in enumerate(graphs):
             assert torch.equal(out, want[(i + k) % len(xs)]), (i, k)
     ops.check_status()
+
+
+def test_torch_ops_give_the_ops_bits(ops):
+    import tri_sds_b200.torch_ops  # noqa: F401
+    tsds = torch.ops.tsds
+    g = _gen(21)
+    x, r, w = _rand(g, 26, 640), _rand(g, 26, 640), _rand(g, 640)
+    no = torch.empty_like(x)
+    want = ops.add_rms_norm_fp8(x, w, residual=r, norm_out=no)
+    got = tsds.add_rms_norm_fp8(x, r, w)
+    for a, b in zip(got, (*want, no)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    wq, ws = tsds.quant_fp8(_rand(g, 1280, 640))
+    q, s = got[0], got[1]
+    assert torch.equal(tsds.linear_fp8(q, s, wq, ws), ops.linear_fp8(q, s, wq, ws))
+    assert torch.equal(tsds.linear_swiglu_fp8(q, s, wq, ws), ops.linear_swiglu_fp8(q, s, wq, ws))
+    res = _rand(g, 26, 1280)
+    assert torch.equal(tsds.linear_residual_fp8(q, s, wq, ws, res), ops.linear_residual_fp8(q, s, wq, ws, res))
+    a, b = _rand(g, 3, 32, 640), _rand(g, 3, 1280, 16)
+    ad = torch.tensor([m % 4 - 1 for m in range(26)], dtype=torch.int32, device=DEV)
+    assert torch.equal(tsds.lora_add(res, x, a, b, ad, None, None, [1024, 256]),
+                       ops.lora_add(res, x, a, b, ad, slices=[1024, 256]))

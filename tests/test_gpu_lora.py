@@ -184,3 +184,23 @@ def test_lora_streams_and_graphs_share_nothing(ops, M):
         for k, (_, _, out, _) in enumerate(graphs):
             assert torch.equal(out, want[(i + k) % 3])
         assert torch.equal(eager, want[(i + 2) % 3])
+
+
+def test_lora_wait_limit_reports_and_recovers(ops):
+    """A wait limit that the two-launch form cannot meet: the call ends, the status is reported, the
+    next call is right."""
+    from tri_sds_b200 import _lib
+    lib = _lib.load()
+    st = _case(2048, 25600, [512], 64, 4, [m // 512 for m in range(2048)])
+    want = ops.lora_add(**st)
+    ops.check_status()
+    limit = lib.tsds_get_wait_limit_ns()
+    try:
+        lib.tsds_set_wait_limit_ns(1)
+        ops.lora_add(**st)
+        with pytest.raises(RuntimeError, match="timed out"):
+            ops.check_status()
+    finally:
+        lib.tsds_set_wait_limit_ns(limit)
+    assert torch.equal(want, ops.lora_add(**st))
+    ops.check_status()

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(THREADS)
       __syncwarp();
       // a CTA without a block of K (K short of 8 blocks) has nothing to wait for
       if (nk > 0) {
-        if (!mbar_wait(&sh.tfull, tphase, p.wait_ns)) give_up(p.l.status, &sh.abort, lane);
+        if (alive && !mbar_wait(&sh.tfull, tphase, p.wait_ns)) give_up(p.l.status, &sh.abort, lane);
         tphase ^= 1;
       }
       __syncwarp();

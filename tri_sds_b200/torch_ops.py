@@ -231,3 +231,57 @@ def allreduce_oneshot(x: Tensor, partial: Tensor, group: int) -> None:
 
 OPS = ("qkv_rope_fused", "verify_attention", "oproj_fused", "mlp_fused", "lm_head_topk", "eagle_fc", "accept_greedy",
        "accept_rejection", "kv_compact", "allreduce_oneshot")
+
+
+# -- 8-bit projections with per-request adapters ------------------------------
+#
+# quant_fp8            rows to e4m3 with a scale per row (weights and activations)
+# add_rms_norm_fp8     residual addition + RMSNorm + e4m3, one launch
+# linear_fp8, linear_residual_fp8, linear_swiglu_fp8
+#                      projections over e4m3 weights and activations
+# lora_add             low-rank adapters of many requests beside a projection
+#
+# No reference counterpart: its projections are bf16 and shared by every request.
+
+@torch.library.custom_op("tsds::quant_fp8", mutates_args=())
+def quant_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x [rows, n] bf16 -> (q [rows, n] float8_e4m3fn, scale [rows] fp32)."""
+    return ops.quant_fp8(x)
+
+
+@torch.library.custom_op("tsds::add_rms_norm_fp8", mutates_args=())
+def add_rms_norm_fp8(x: Tensor, residual: Tensor, norm_w: Tensor,
+                     eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """r = x + residual -> (q, scale) of RMSNorm(r), r, and RMSNorm(r) in
+    bf16 (what adapters beside the projection read)."""
+    norm = torch.empty_like(x)
+    q, s, r = ops.add_rms_norm_fp8(x, norm_w, residual=residual, eps=eps, norm_out=norm)
+    return q, s, r, norm
+
+
+@torch.library.custom_op("tsds::linear_fp8", mutates_args=())
+def linear_fp8(x: Tensor, x_scale: Tensor, w: Tensor, w_scale: Tensor) -> Tensor:
+    """(x * x_scale) @ (w * w_scale)^T, bf16 [M, n_out]."""
+    return ops.linear_fp8(x, x_scale, w, w_scale)
+
+
+@torch.library.custom_op("tsds::linear_residual_fp8", mutates_args=())
+def linear_residual_fp8(x: Tensor, x_scale: Tensor, w: Tensor, w_scale: Tensor, res: Tensor) -> Tensor:
+    """res + the 8-bit projection, rounded once."""
+    return ops.linear_residual_fp8(x, x_scale, w, w_scale, res)
+
+
+@torch.library.custom_op("tsds::linear_swiglu_fp8", mutates_args=())
+def linear_swiglu_fp8(x: Tensor, x_scale: Tensor, w_gate_up: Tensor, w_scale: Tensor) -> Tensor:
+    """silu(gate) * up of the 8-bit projections, w_gate_up = [gate; up]."""
+    return ops.linear_swiglu_fp8(x, x_scale, w_gate_up, w_scale)
+
+
+@torch.library.custom_op("tsds::lora_add", mutates_args=())
+def lora_add(y: Tensor, x: Tensor, lora_a: Tensor, lora_b: Tensor, adapter: Tensor, scale: Optional[Tensor] = None,
+             ranks: Optional[Tensor] = None, slices: Optional[list[int]] = None) -> Tensor:
+    """y + scale[a] * B_a (A_a x) per row, a = adapter[row] (negative: none)."""
+    return ops.lora_add(y, x, lora_a, lora_b, adapter, scale=scale, ranks=ranks, slices=slices)
+
+
+PROJECTION_OPS = ("quant_fp8", "add_rms_norm_fp8", "linear_fp8", "linear_residual_fp8", "linear_swiglu_fp8", "lora_add")
