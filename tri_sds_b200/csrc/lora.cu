@@ -245,13 +245,26 @@ struct First {
     // k is summed in the order the 16-byte loads give it: lane q of a row
     // holds k = 8q .. 8q+7 of a chunk, elements 0-3 in the first step and 4-7
     // in the second, the same for both operands
-    const int chunks = (p.K + 31) / 32;
-    for (int c0 = rank * WARPS + warp; c0 < chunks; c0 += CL * WARPS * U) {
+    const int chunks = (p.K + 31) / 32, lo = rank * chunks / CL, hi = (rank + 1) * chunks / CL;
+    if (hi - lo > WARPS * U && hi * 32 <= p.K) {
+      // several rounds of loads: this CTA's part of every row goes to L2 at once, so
+      // that only the first round waits for DRAM
+      const uint32_t bytes = (uint32_t)(hi - lo) * 64;
+      for (int i = tid; i < nt * 8 + TR; i += THREADS) {
+        const int u = t0 + i / 8, s = u / ad.nr8, r = (u - s * ad.nr8) * 8 + i % 8, m = row0 + i - nt * 8;
+        if (i < nt * 8 && r < ad.ra)
+          prefetch_l2(p.a + ((int64_t)ad.id * p.S * p.R + s * p.R + r) * p.K + lo * 32, bytes);
+        else if (i >= nt * 8 && m < p.M)
+          prefetch_l2(p.x + (int64_t)m * p.ldx + lo * 32, bytes);
+      }
+      __syncwarp();
+    }
+    for (int c0 = lo + warp; c0 < hi; c0 += WARPS * U) {
       uint4 xv[U][2], av[U][NT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int k = (c0 + u * CL * WARPS) * 32;
-        const bool in = k + 8 * q < p.K;
+        const int c = c0 + u * WARPS, k = c * 32;
+        const bool in = c < hi && k + 8 * q < p.K;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
           av[u][i] = in && ar[i] >= 0 ? ldg16(a_id + (int64_t)ar[i] * p.K + k) : make_uint4(0, 0, 0, 0);
