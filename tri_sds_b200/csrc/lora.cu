@@ -366,9 +366,9 @@ int launch_lora(LoraArgs p, cudaStream_t stream) {
   const int st = tsds_smem_limit_once(lora_kernel<F>, most, limit_set);
   if (st != TSDS_OK) return st;
   const int tiles = (p.M + TR - 1) / TR;
-  // a cluster per adapter of a tile while the grid stays within ~1000 CTAs
+  // a cluster per adapter of a tile while the grid stays within ~500 CTAs
   // (clusters without one leave at once); beyond that a cluster takes several
-  int slots = 128 / tiles;
+  int slots = 60 / tiles;
   slots = slots < 1 ? 1 : (slots > TR + 1 ? TR + 1 : slots);
   if (slots > p.n_adapters + 1) slots = p.n_adapters + 1;
   p.slots = slots;
@@ -437,11 +437,12 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
     TSDS_RETURN_IF(!tsds_aligned16(workspace), TSDS_E_ALIGN);
     return tsds_lora_tc(p, workspace, stream);
   }
-  // One tile of rows is a matter of latency: many warps and loads per CTA (q/k/v
-  // adapters of 8 one-token requests 11.2 us, 14.2 with the smaller CTAs).  With
-  // several tiles two smaller CTAs per SM overlap (8 x 26 rows 14.5 us, 21.8 with
-  // the larger ones).
-  if (M > TR) return launch_lora<First<8, 1, 8, 2>>(p, stream);
+  // Where a cluster for every adapter of every tile fits the SMs at once the call
+  // is a matter of latency: many warps and loads per CTA (q/k/v adapters of 8
+  // one-token requests 11.2 us, 14.2 with the smaller CTAs).  With more of them two
+  // smaller CTAs per SM overlap (8 x 26 rows 14.4 us, 21.7 with the larger ones).
+  const int most = (M + TR - 1) / TR * (n_adapters < TR ? n_adapters : TR);
+  if (most > tsds_tc_num_sms() / CL) return launch_lora<First<8, 1, 8, 2>>(p, stream);
   if (n_slices * R <= 16) return launch_lora<First<2, 4, 16, 1>>(p, stream);
   return launch_lora<First<8, 2, 12, 1>>(p, stream);
 }
