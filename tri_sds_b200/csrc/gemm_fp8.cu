@@ -118,8 +118,11 @@ __device__ __forceinline__ bool epi_all(bool ok) {
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
-template <int EPI, int CG>   // CG: CTAs per unit
-__global__ void __launch_bounds__(THREADS)
+// CG: CTAs per unit.  One CTA per SM as the register target: with ptxas's own
+// choice (56 registers for the residual epilogue) the loads of the split
+// epilogue no longer go out together (O at 128 rows 17.6 us instead of 15.9).
+template <int EPI, int CG>
+__global__ void __launch_bounds__(THREADS, 1)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, F8Args p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -191,27 +194,38 @@ __global__ void __launch_bounds__(THREADS)
     }
     return w;
   };
-  auto finish = [&](const Out& w, int m, const float4 (&acc)[2]) {
-    const float sx = p.sx[m];
-    const float a4[4] = {acc[0].x, acc[0].y, acc[0].z, acc[0].w};
-    float rv[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+  // what a row's outputs take from global memory, loaded ahead of its sums: the
+  // residual may be the output, so a load cannot pass an earlier row's store
+  struct In {
+    float sx;
+    uint2 res;
+  };
+  auto load_in = [&](const Out& w, int m, bool in) {
+    In v = {0.f, make_uint2(0, 0)};
+    if (!in || w.left <= 0) return v;
+    v.sx = p.sx[m];
     if constexpr (EPI == EPI_RESIDUAL) {
       const bf16* rp = p.res + (int64_t)m * p.res_ld + w.j;
       if (w.vec) {
-        const uint2 u = *reinterpret_cast<const uint2*>(rp);
-        rv[0] = bf_lo(u.x), rv[1] = bf_hi(u.x), rv[2] = bf_lo(u.y), rv[3] = bf_hi(u.y);
+        v.res = *reinterpret_cast<const uint2*>(rp);
       } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < w.left) rv[i] = bf2f(rp[i]);
+        const uint16_t* r16 = reinterpret_cast<const uint16_t*>(rp);
+        v.res.x = r16[0] | (w.left > 1 ? (uint32_t)r16[1] << 16 : 0u);
+        v.res.y = (w.left > 2 ? r16[2] : 0u) | (w.left > 3 ? (uint32_t)r16[3] << 16 : 0u);
       }
     }
+    return v;
+  };
+  auto finish = [&](const Out& w, int m, const float4 (&acc)[2], const In& in) {
+    const float a4[4] = {acc[0].x, acc[0].y, acc[0].z, acc[0].w};
+    const float rv[4] = {bf_lo(in.res.x), bf_hi(in.res.x), bf_lo(in.res.y), bf_hi(in.res.y)};
+    float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o[i] = a4[i] * sx * w.sw[0][i];
+      o[i] = a4[i] * in.sx * w.sw[0][i];
       if constexpr (SW) {
         const float b4[4] = {acc[1].x, acc[1].y, acc[1].z, acc[1].w};
-        o[i] = silu(o[i]) * (b4[i] * sx * w.sw[1][i]);
+        o[i] = silu(o[i]) * (b4[i] * in.sx * w.sw[1][i]);
       }
       if constexpr (EPI == EPI_RESIDUAL) o[i] += rv[i];
     }
@@ -222,6 +236,17 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (i < w.left) op[i] = f2bf(o[i]);
+    }
+  };
+
+  // The residual's lines of rows m .. m + rows - 1 of a tile into L2, by the 128
+  // epilogue threads while the tensor cores work
+  auto prefetch_res = [&](int tile, int m, int rows) {
+    if constexpr (EPI == EPI_RESIDUAL) {
+      const int j = tile * TILE_J + (threadIdx.x & 1) * 64;
+      if (j >= p.n_out) return;
+      for (int i = ((int)threadIdx.x - 64) >> 1; i < rows; i += 64)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.res + (int64_t)(m + i) * p.res_ld + j));
     }
   };
 
@@ -329,6 +354,7 @@ __global__ void __launch_bounds__(THREADS)
     for (int u = first_unit; u < p.units; u += unit_step) {
       const Out w = out_of(tile_of(u), g4);
       const int m0 = row_of(u), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+      prefetch_res(tile_of(u), m0, rows);
       // the four warps go on together or not at all
       const bool ok = mbar_wait(&sh.tfull[buf], tphase, p.wait_ns);
       if (!ok) {
@@ -339,6 +365,12 @@ __global__ void __launch_bounds__(THREADS)
       __syncwarp();
       tc_fence_after();
       const uint32_t at = tmem + buf * p.tmem_cols + ((uint32_t)(quarter * 32) << 16);
+      In in[16 / STEP];
+      auto load_chunk = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 16; i += STEP) in[i / STEP] = load_in(w, m0 + c + i + et / G, c + i + et / G < rows);
+      };
+      load_chunk(0);
       for (int c = 0; c < rows; c += 16) {
         float v[16];
         tmem_ld16(at + c, v);
@@ -355,9 +387,10 @@ __global__ void __launch_bounds__(THREADS)
               float4 acc[2];
               acc[0] = *reinterpret_cast<const float4*>(from + mc * TILE_J);
               if constexpr (SW) acc[1] = *reinterpret_cast<const float4*>(from + mc * TILE_J + 64);
-              finish(w, m0 + c + mc, acc);
+              finish(w, m0 + c + mc, acc, in[i / STEP]);
             }
           }
+          if (c + 16 < rows) load_chunk(c + 16);
         }
         __syncwarp();
       }
@@ -377,6 +410,11 @@ __global__ void __launch_bounds__(THREADS)
   }
   if (p.C > 1) {
     pdl_wait();
+    if (warp >= 2) {   // this CTA's share of the rows (of the first chunk)
+      const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+      const int cn = rows < p.chunk ? rows : p.chunk, lo = rank * cn / p.C;
+      prefetch_res(tile_of(first_unit), m0 + lo, (rank + 1) * cn / p.C - lo);
+    }
     __syncwarp();
     // tfull completes when every MMA has, so the ring is free for the partials
     if (!mbar_wait(&sh.tfull[0], 0, p.wait_ns)) {
@@ -423,6 +461,7 @@ __global__ void __launch_bounds__(THREADS)
         // this CTA's token rows, from every CTA's partials in rank order
         const int hi = (rank + 1) * cn / p.C;
         for (int mc = rank * cn / p.C + (int)threadIdx.x / G; mc < hi; mc += STEP) {
+          const In in = load_in(w, m0 + c0 + mc, true);
           const uint32_t at = smem_u32(part + mc * TILE_J + g4);
           float4 acc[2];
 #pragma unroll
@@ -436,7 +475,7 @@ __global__ void __launch_bounds__(THREADS)
             for (int q = 1; q < MAX_C; ++q)
               if (q < p.C) acc[h] = add4(acc[h], f[q]);
           }
-          finish(w, m0 + c0 + mc, acc);
+          finish(w, m0 + c0 + mc, acc, in);
         }
       }
       cluster_barrier();   // the peers are done with this CTA's partials
