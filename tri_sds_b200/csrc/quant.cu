@@ -16,6 +16,7 @@
 // Sums and maxima are fp32; max.NaN keeps a NaN, so a row that holds one
 // gets a NaN scale and NaN values.
 #include "common.cuh"
+#include "linear.cuh"
 
 using namespace tsds;
 
@@ -23,7 +24,6 @@ namespace {
 
 constexpr float kTop = 448.0f;              // largest e4m3 value
 constexpr float kTiny = 7.88860905e-31f;    // 2^-100: smallest magnitude a row is scaled to
-constexpr int VMAX = 4;                     // 16-byte vectors a thread keeps in registers
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -105,10 +105,10 @@ __device__ __forceinline__ void store8(const QuantArgs& a, uint8_t* qrow, bf16* 
   }
 }
 
-// One CTA of NT threads per row.  Rows of at most NT * VMAX vectors are read
+// One CTA of NT threads per row.  Rows of at most NT * VMAX 16-byte vectors are read
 // once and kept in registers; longer ones are read a second time (from
 // res_out when there is a residual).
-template <bool NORM, int NT>
+template <bool NORM, int NT, int VMAX>
 __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
   __shared__ float red_s[NT / 32], red_m[NT / 32];
   pdl_trigger();
@@ -205,15 +205,22 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
   }
 }
 
+template <bool NORM, int NT, int VMAX>
+int launch(const QuantArgs& a, int rows, cudaStream_t stream) {
+  tsds_launch(quant_rows_kernel<NORM, NT, VMAX>, dim3(rows), dim3(NT), 0, stream, a);
+  return tsds_launch_status();
+}
+
+// Rows of up to 8192 elements: 256 threads.  Longer ones: 1024 threads where
+// the rows are few and one row's time is what counts; with many rows half as
+// many threads with twice the vectors each keep more loads in flight per SM
+// (quantising 5809 rows of 9024: 55 us with 1024 threads).
 template <bool NORM>
 int launch_rows(const QuantArgs& a, int rows, cudaStream_t stream) {
-  // 256 threads keep rows of up to 8192 elements in registers, 1024 threads
-  // rows of up to 32768
-  if (a.n <= 256 * VMAX * 8)
-    tsds_launch(quant_rows_kernel<NORM, 256>, dim3(rows), dim3(256), 0, stream, a);
-  else
-    tsds_launch(quant_rows_kernel<NORM, 1024>, dim3(rows), dim3(1024), 0, stream, a);
-  return tsds_launch_status();
+  if (a.n <= 8192) return launch<NORM, 256, 4>(a, rows, stream);
+  if (rows < 2 * tsds_tc_num_sms() || a.n > 32768) return launch<NORM, 1024, 4>(a, rows, stream);
+  if (a.n <= 16384) return launch<NORM, NORM ? 512 : 256, NORM ? 4 : 8>(a, rows, stream);
+  return launch<NORM, 512, 8>(a, rows, stream);
 }
 
 }  // namespace
