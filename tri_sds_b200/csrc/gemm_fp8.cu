@@ -35,6 +35,8 @@
 #include "linear.cuh"
 #include "tc_core.cuh"
 
+#include <type_traits>
+
 using namespace tsds;
 using namespace tsds::tc;
 
@@ -48,7 +50,7 @@ constexpr int RING = 8;                  // most stages
 constexpr int MAX_C = 8;                 // largest portable cluster
 constexpr int SMEM_SM = 233472;          // 228 KB per SM
 constexpr int SMEM_CTA = 220 * 1024;     // dynamic shared memory a CTA may ask for
-constexpr int STAGING = 2 * 16 * TILE_J * 4;   // output staging of a persistent CTA
+constexpr int STAGING = 32 * TILE_J * 4;   // output staging of a persistent CTA
 constexpr int SMEM_SIDE = 2048;          // static shared memory + the system's 1 KB per CTA
 
 struct F8Args {
@@ -118,11 +120,13 @@ __device__ __forceinline__ bool epi_all(bool ok) {
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
 
-// CG: CTAs per unit.  One CTA per SM as the register target: with ptxas's own
-// choice (56 registers for the residual epilogue) the loads of the split
-// epilogue no longer go out together (O at 128 rows 17.6 us instead of 15.9).
-template <int EPI, int CG>
-__global__ void __launch_bounds__(THREADS, 1)
+// CG: CTAs per unit; SPLIT: a unit's K over a cluster.  One CTA per SM as the
+// register target: with ptxas's own choice (56 registers for the residual
+// epilogue) the loads of the split epilogue no longer go out together (O at 128
+// rows 17.6 us instead of 15.9).  Whole units of one CTA, which have few rows,
+// must leave room for three CTAs per SM (gate/up at 26 rows 48 us with two).
+template <int EPI, int CG, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, F8Args p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -173,71 +177,75 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* b_smem = smem + p.stages * A_BYTES;
   pdl_trigger();
   int issued = 0;
-  // what a thread of the epilogue works on: four channels j .. j+3 of the tile
-  // (their scales in registers) and every token row that is its turn
-  constexpr int G = SW ? 16 : 32;
+  // What a thread of the epilogue works on: four channels of the tile (their
+  // scales in registers) and every token row that is its turn.  The channels
+  // are adjacent (8-byte accesses) where the buffers' alignment allows; else
+  // `spread` apart, so that neighbouring threads' 2-byte accesses still are.
   struct Out {
-    int j, left;      // first channel; channels inside the output
+    int j, step;      // first channel, distance of the next
+    int count;        // channels inside the output
     bool vec;         // 8-byte accesses
     float sw[SW ? 2 : 1][4];
   };
-  auto out_of = [&](int tile, int g4) {
+  auto out_of = [&](int tile, int first, int t, int spread) {
     Out w;
-    w.j = tile * ROWS + g4;
-    w.left = p.n_out - w.j;
-    w.vec = w.left >= 4 && (p.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 &&
+    const int base = tile * ROWS, inside = p.n_out - base < ROWS ? p.n_out - base : ROWS;
+    w.vec = (p.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && inside % 4 == 0 &&
             (EPI != EPI_RESIDUAL || ((p.res_ld % 4) == 0 && (reinterpret_cast<uintptr_t>(p.res) & 7) == 0));
+    w.step = w.vec ? 1 : spread;
+    w.j = base + first + (spread == 1 || w.vec ? t * 4 : t);
+    const int left = base + inside - w.j;
+    w.count = left <= 0 ? 0 : ((left + w.step - 1) / w.step < 4 ? (left + w.step - 1) / w.step : 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w.sw[0][i] = i < w.left ? p.sw[w.j + i] : 0.f;
-      if constexpr (SW) w.sw[1][i] = i < w.left ? p.sw[p.n_out + w.j + i] : 0.f;
+      w.sw[0][i] = i < w.count ? p.sw[w.j + i * w.step] : 0.f;
+      if constexpr (SW) w.sw[1][i] = i < w.count ? p.sw[p.n_out + w.j + i * w.step] : 0.f;
     }
     return w;
   };
-  // what a row's outputs take from global memory, loaded ahead of its sums: the
-  // residual may be the output, so a load cannot pass an earlier row's store
-  struct In {
-    float sx;
-    uint2 res;
-  };
-  auto load_in = [&](const Out& w, int m, bool in) {
-    In v = {0.f, make_uint2(0, 0)};
-    if (!in || w.left <= 0) return v;
-    v.sx = p.sx[m];
+  // A row's residual, loaded ahead of its sums: the residual may be the output,
+  // so a load cannot pass an earlier row's store.  FULL: all four channels are
+  // inside the output; a warp alone on its scheduler pays each branch in full.
+  auto load_res = [&](auto full, auto vec, const Out& w, int m) {
+    uint2 v = make_uint2(0, 0);
     if constexpr (EPI == EPI_RESIDUAL) {
       const bf16* rp = p.res + (int64_t)m * p.res_ld + w.j;
-      if (w.vec) {
-        v.res = *reinterpret_cast<const uint2*>(rp);
+      if (vec) {
+        if (full || w.count > 0) v = *reinterpret_cast<const uint2*>(rp);
       } else {
         const uint16_t* r16 = reinterpret_cast<const uint16_t*>(rp);
-        v.res.x = r16[0] | (w.left > 1 ? (uint32_t)r16[1] << 16 : 0u);
-        v.res.y = (w.left > 2 ? r16[2] : 0u) | (w.left > 3 ? (uint32_t)r16[3] << 16 : 0u);
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = full || i < w.count ? r16[i * w.step] : 0;
+        v = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
       }
     }
     return v;
   };
-  auto finish = [&](const Out& w, int m, const float4 (&acc)[2], const In& in) {
+  auto finish = [&](auto full, auto vec, const Out& w, int m, const float4 (&acc)[2], float sx, uint2 res) {
     const float a4[4] = {acc[0].x, acc[0].y, acc[0].z, acc[0].w};
-    const float rv[4] = {bf_lo(in.res.x), bf_hi(in.res.x), bf_lo(in.res.y), bf_hi(in.res.y)};
+    const float rv[4] = {bf_lo(res.x), bf_hi(res.x), bf_lo(res.y), bf_hi(res.y)};
     float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o[i] = a4[i] * in.sx * w.sw[0][i];
+      o[i] = a4[i] * sx * w.sw[0][i];
       if constexpr (SW) {
         const float b4[4] = {acc[1].x, acc[1].y, acc[1].z, acc[1].w};
-        o[i] = silu(o[i]) * (b4[i] * in.sx * w.sw[1][i]);
+        o[i] = silu(o[i]) * (b4[i] * sx * w.sw[1][i]);
       }
       if constexpr (EPI == EPI_RESIDUAL) o[i] += rv[i];
     }
     bf16* op = p.out + (int64_t)m * p.ldo + w.j;
-    if (w.vec) {
-      *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
+    if (vec) {
+      if (full || w.count > 0) *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3]));
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i < w.left) op[i] = f2bf(o[i]);
+        if (full || i < w.count) op[i * w.step] = f2bf(o[i]);
     }
   };
+  using Yes = std::true_type;
+  using No = std::false_type;
 
   // The residual's lines of rows m .. m + rows - 1 of a tile into L2, by the 128
   // epilogue threads while the tensor cores work
@@ -341,20 +349,57 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) atomicExch(p.status, TSDS_E_TIMEOUT);
       *(volatile int*)&sh.abort = 1;
     }
-  } else if (p.C == 1) {
-    // ---- epilogue of whole units: 16 token rows at a time through a small
-    // double-buffered staging area, so that stores are whole lines ----
+  } else if constexpr (!SPLIT) {
+    // ---- epilogue of whole units: each warp transposes 32 token rows at a time of
+    // its 32 channels through 4 KB of its own, so that stores are 64-byte runs
+    // and no warp waits for another (SwiGLU: a gate warp and its up warp share
+    // 8 KB and take half of the rows each).  The next 32 columns of TMEM and
+    // the residuals of the next 32 rows are on their way meanwhile.  With one
+    // staging area for the block and a block barrier per 16 rows a unit of 256
+    // rows took 8 us, more than its main loop up to K = 4096. ----
     pdl_wait();
-    const int quarter = warp & 3;   // the TMEM lanes this warp may read
-    const int et = threadIdx.x - 64, g4 = et % G * 4;
-    constexpr int STEP = 128 / G;
-    float* stg = reinterpret_cast<float*>(smem + p.out_off);
+    constexpr int PASS = SW ? 4 : 8;   // of 4 rows each, 8 threads to a row
+    constexpr int BATCH = CG == 2 ? 4 : 1;   // passes whose sums a thread holds at once
+    const int quarter = warp & 3;      // the TMEM lanes this warp may read
+    const int strip = SW ? quarter & 1 : quarter;
+    const int mine = SW ? (quarter >> 1) * 16 + lane / 8 : lane / 8;   // row of the first pass
+    float* from = reinterpret_cast<float*>(smem + p.out_off) + strip * (SW ? 2048 : 1024);
+    float* to = from + (SW ? (quarter >> 1) * 1024 : 0) + lane;
+    auto strip_sync = [&] {
+      if (!SW)
+        __syncwarp();
+      else if (strip == 0)
+        asm volatile("bar.sync 2, 64;" ::: "memory");
+      else
+        asm volatile("bar.sync 3, 64;" ::: "memory");
+    };
     int buf = 0;
     uint32_t tphase = 0;
     for (int u = first_unit; u < p.units; u += unit_step) {
-      const Out w = out_of(tile_of(u), g4);
+      const Out w = out_of(tile_of(u), strip * 32, lane % 8, 8);
       const int m0 = row_of(u), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
       prefetch_res(tile_of(u), m0, rows);
+      const bool full = __all_sync(0xffffffffu, w.count == 4);
+      struct Rows {   // what 32 rows take from global memory
+        float sx;     // of row `lane`
+        uint2 res[PASS];
+      } in0, in1;
+      auto load_rows = [&](Rows& in, int c) {
+        in.sx = c + lane < rows ? p.sx[m0 + c + lane] : 0.f;
+        const int m = m0 + c + mine;
+        if (full && w.vec && c + 32 <= rows) {
+#pragma unroll
+          for (int i = 0; i < PASS; ++i) in.res[i] = load_res(Yes(), Yes(), w, m + i * 4);
+        } else if (full && c + 32 <= rows) {
+#pragma unroll
+          for (int i = 0; i < PASS; ++i) in.res[i] = load_res(Yes(), No(), w, m + i * 4);
+        } else {
+#pragma unroll
+          for (int i = 0; i < PASS; ++i)
+            if (c + mine + i * 4 < rows) in.res[i] = load_res(No(), w.vec, w, m + i * 4);
+        }
+      };
+      load_rows(in0, 0);
       // the four warps go on together or not at all
       const bool ok = mbar_wait(&sh.tfull[buf], tphase, p.wait_ns);
       if (!ok) {
@@ -365,42 +410,59 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       tc_fence_after();
       const uint32_t at = tmem + buf * p.tmem_cols + ((uint32_t)(quarter * 32) << 16);
-      In in[16 / STEP];
-      auto load_chunk = [&](int c) {
+      uint32_t v[32];
+      tmem_request32(at, v);
+      // (TMEM columns come in powers of two from 32: those past the last row are there)
+      auto do_rows = [&](const Rows& in, Rows& next, int c) {
+        tmem_wait32(v);
+        if (c + 32 >= rows) {   // this warp has read its part of the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2)
+              mbar_arrive_remote(mapa_shared(smem_u32(&sh.tempty[buf]), lead));   // the leader's MMAs reuse it
+            else
+              mbar_arrive(&sh.tempty[buf]);
+          }
+        }
+        strip_sync();   // the rows before have been read
 #pragma unroll
-        for (int i = 0; i < 16; i += STEP) in[i / STEP] = load_in(w, m0 + c + i + et / G, c + i + et / G < rows);
-      };
-      load_chunk(0);
-      for (int c = 0; c < rows; c += 16) {
-        float v[16];
-        tmem_ld16(at + c, v);
-        float* to = stg + (c & 16) * TILE_J + quarter * 32 + lane;
+        for (int i = 0; i < 32; ++i) to[i * 32] = __uint_as_float(v[i]);
+        strip_sync();
+        if (c + 32 < rows) {
+          tmem_request32(at + c + 32, v);
+          load_rows(next, c + 32);
+        }
+        auto rest = [&](auto whole, auto vec) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) to[i * TILE_J] = v[i];
-        epi_bar();
-        const float* from = stg + (c & 16) * TILE_J + g4;
-        if (w.left > 0) {
+          for (int i0 = 0; i0 < PASS; i0 += BATCH) {
+            float4 acc[BATCH][2];
 #pragma unroll
-          for (int i = 0; i < 16; i += STEP) {
-            const int mc = i + et / G;
-            if (c + mc < rows) {
-              float4 acc[2];
-              acc[0] = *reinterpret_cast<const float4*>(from + mc * TILE_J);
-              if constexpr (SW) acc[1] = *reinterpret_cast<const float4*>(from + mc * TILE_J + 64);
-              finish(w, m0 + c + mc, acc, in[i / STEP]);
+            for (int i = 0; i < BATCH; ++i)
+#pragma unroll
+              for (int h = 0; h < (SW ? 2 : 1); ++h) {
+                const float* a = from + h * 1024 + (mine + (i0 + i) * 4) * 32 + (vec ? lane % 8 * 4 : lane % 8);
+                acc[i][h] = vec ? *reinterpret_cast<const float4*>(a) : make_float4(a[0], a[8], a[16], a[24]);
+              }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              const int mc = mine + (i0 + i) * 4;
+              const float sx = __shfl_sync(0xffffffffu, in.sx, mc);
+              if (whole || c + mc < rows) finish(whole, vec, w, m0 + c + mc, acc[i], sx, in.res[i0 + i]);
             }
           }
-          if (c + 16 < rows) load_chunk(c + 16);
-        }
-        __syncwarp();
-      }
-      tc_fence_before();
-      epi_bar();   // the staging area is free for the next unit
-      if (lane == 0) {
-        if constexpr (CG == 2)
-          mbar_arrive_remote(mapa_shared(smem_u32(&sh.tempty[buf]), lead));   // the leader's MMAs reuse it
+        };
+        if (full && w.vec && c + 32 <= rows)
+          rest(Yes(), Yes());
+        else if (full && c + 32 <= rows)
+          rest(Yes(), No());
         else
-          mbar_arrive(&sh.tempty[buf]);
+          rest(No(), w.vec);
+        __syncwarp();
+      };
+      for (int c = 0; c < rows; c += 64) {
+        do_rows(in0, in1, c);
+        if (c + 32 < rows) do_rows(in1, in0, c + 32);
       }
       if (++buf == p.bufs) {
         buf = 0;
@@ -408,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   }
-  if (p.C > 1) {
+  if constexpr (SPLIT) {
     pdl_wait();
     if (warp >= 2) {   // this CTA's share of the rows (of the first chunk)
       const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
@@ -436,12 +498,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     __syncthreads();
   }
-  if (p.C > 1) {
+  if constexpr (SPLIT) {
     // ---- epilogue of a split unit: token rows in chunks that fit the ring, partials [chunk][128] fp32 ----
     float* part = reinterpret_cast<float*>(smem);
+    constexpr int G = SW ? 16 : 32, STEP = THREADS / G;
     const int g4 = threadIdx.x % G * 4;
-    constexpr int STEP = THREADS / G;
-    const Out w = out_of(tile_of(first_unit), g4);
+    const Out w = out_of(tile_of(first_unit), 0, threadIdx.x % G, 1);
     const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
     for (int c0 = 0; c0 < rows; c0 += p.chunk) {
       const int cn = rows - c0 < p.chunk ? rows - c0 : p.chunk;
@@ -457,11 +519,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       cluster_barrier();
-      if (alive && w.left > 0) {
+      if (alive && w.count > 0) {
         // this CTA's token rows, from every CTA's partials in rank order
         const int hi = (rank + 1) * cn / p.C;
         for (int mc = rank * cn / p.C + (int)threadIdx.x / G; mc < hi; mc += STEP) {
-          const In in = load_in(w, m0 + c0 + mc, true);
+          const uint2 res = load_res(No(), w.vec, w, m0 + c0 + mc);
+          const float sx = p.sx[m0 + c0 + mc];
           const uint32_t at = smem_u32(part + mc * TILE_J + g4);
           float4 acc[2];
 #pragma unroll
@@ -475,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int q = 1; q < MAX_C; ++q)
               if (q < p.C) acc[h] = add4(acc[h], f[q]);
           }
-          finish(w, m0 + c0 + mc, acc, in);
+          finish(No(), w.vec, w, m0 + c0 + mc, acc, sx, res);
         }
       }
       cluster_barrier();   // the peers are done with this CTA's partials
@@ -540,16 +603,17 @@ Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas,
   return h;
 }
 
-template <int EPI, int CG>
+template <int EPI, int CG, bool SPLIT>
 int launch(const CUtensorMap& amap, const CUtensorMap& bmap, const F8Args& p, unsigned grid, size_t smem,
            cudaStream_t stream) {
   static tsds_device_flags limit_set;
-  const int st = tsds_smem_limit_once(f8_gemm_kernel<EPI, CG>, SMEM_CTA, limit_set);
+  const int st = tsds_smem_limit_once(f8_gemm_kernel<EPI, CG, SPLIT>, SMEM_CTA, limit_set);
   if (st != TSDS_OK) return st;
   if (p.C * CG > 1)
-    tsds_launch_cluster(f8_gemm_kernel<EPI, CG>, dim3(grid), dim3(THREADS), smem, stream, p.C * CG, amap, bmap, p);
+    tsds_launch_cluster(f8_gemm_kernel<EPI, CG, SPLIT>, dim3(grid), dim3(THREADS), smem, stream, p.C * CG, amap, bmap,
+                        p);
   else
-    tsds_launch(f8_gemm_kernel<EPI, CG>, dim3(grid), dim3(THREADS), smem, stream, amap, bmap, p);
+    tsds_launch(f8_gemm_kernel<EPI, CG, SPLIT>, dim3(grid), dim3(THREADS), smem, stream, amap, bmap, p);
   return tsds_launch_status();
 }
 
@@ -594,8 +658,11 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   st = tsds_make_tmap_2d_u8(&bmap, x, K, p.M, ldx, KB, p.npad / best.CG);
   if (st != TSDS_OK) return st;
   const unsigned grid = (unsigned)(best.grid * best.CG);
-  return best.CG == 2 ? launch<EPI, 2>(amap, bmap, p, grid, smem, stream)
-                      : launch<EPI, 1>(amap, bmap, p, grid, smem, stream);
+  if (best.CG == 2)
+    return p.C > 1 ? launch<EPI, 2, true>(amap, bmap, p, grid, smem, stream)
+                   : launch<EPI, 2, false>(amap, bmap, p, grid, smem, stream);
+  return p.C > 1 ? launch<EPI, 1, true>(amap, bmap, p, grid, smem, stream)
+                 : launch<EPI, 1, false>(amap, bmap, p, grid, smem, stream);
 }
 
 int check(const void* x, int ldx, const float* sx, const void* w, const float* sw, const void* out, int ldo, int M,
