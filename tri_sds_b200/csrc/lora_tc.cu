@@ -23,6 +23,8 @@
 #include "lora.cuh"
 #include "tc_core.cuh"
 
+#include <type_traits>
+
 using namespace tsds;
 using namespace tsds::tc;
 using namespace tsds::lora;
@@ -54,6 +56,18 @@ struct ShrinkShared {
   int abort;
 };
 
+// TMEM columns for the CTA, by one whole warp, before anything else: the SM's
+// next CTA does not start until this one has given its permit to allocate back
+// (taken after the rows' grouping it held every second CTA up for 5 us).
+__device__ __forceinline__ void tmem_take(uint32_t* to, int columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(to)), "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_give(uint32_t tmem, int columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+
 __device__ __forceinline__ void give_up(int32_t* status, int* abort, int lane) {
   if (lane == 0) atomicExch(status, TSDS_E_TIMEOUT);
   *(volatile int*)abort = 1;
@@ -67,6 +81,7 @@ __global__ void __launch_bounds__(THREADS)
   __shared__ ShrinkShared sh;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
+  if (warp == 1) tmem_take(&sh.tmem, p.tmem_cols);
   // every block's first adapter before any block's second: clusters without one come last
   const int unit = blockIdx.x / CL, slot = unit / p.blocks, row0 = (unit - slot * p.blocks) * p.nt;
   if (warp == 0 && elect_one()) {
@@ -81,20 +96,16 @@ __global__ void __launch_bounds__(THREADS)
     sh.abort = 0;
     fence_barrier_init();
   }
+  tc_fence_before();
   pdl_wait();
   pdl_trigger();   // after the wait: expand reads what comes before this kernel without one
   group_rows(p.l, sh.tile, row0, p.nt, rank == 0 && slot == 0, false);
-  // a cluster whose turn never comes leaves before it takes TMEM
-  if (__popcll(sh.tile.leads) <= slot) return;
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(p.tmem_cols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  tc_fence_after();   // (group_rows ends with a barrier)
   const uint32_t tmem = sh.tmem;
+  if (__popcll(sh.tile.leads) <= slot) {   // a cluster whose turn never comes
+    if (warp == 1) tmem_give(tmem, p.tmem_cols);
+    return;
+  }
   float* part = reinterpret_cast<float*>(smem);   // [nt][128], in the ring once it is free
   const int k_lo = rank * p.KT / CL, nk = (rank + 1) * p.KT / CL - k_lo;
   int s = 0, issued = 0;                 // ring position, blocks so far (warps 0 and 1)
@@ -235,7 +246,7 @@ __global__ void __launch_bounds__(THREADS)
   }
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
+    tmem_give(tmem, p.tmem_cols);
   }
 }
 
@@ -243,17 +254,19 @@ constexpr int XN = 64;                      // token rows of an expand unit
 constexpr int X_THREADS = 320;              // TMA warp, MMA warp, two groups of four epilogue warps
 constexpr int B_TILE = TILE_J * 128;        // 128 channels x 64 ranks
 constexpr int T_TILE = XN * 128;            // 64 token rows x 64 ranks
-constexpr int X_STAGING = 2 * 16 * TILE_J * (int)sizeof(float);
+constexpr int X_LD = 36;                    // padded row of 32 staged channels: 16-byte reads of two rows in all banks
+constexpr int X_STAGING = 8 * 16 * X_LD * (int)sizeof(float);
 
 struct ExpandArgs {
   LoraArgs l;
-  int ld_t, Rp, blocks, tiles, step, kb;    // step: CTAs that share a block's channel tiles; kb: blocks of 64 ranks
+  int ld_t, Rp, blocks, tiles, step, kb;    // step: CTAs that share a block's items; kb: blocks of 64 ranks
   int first_tile[MAX_SLICES + 1];           // channel tiles where the slices begin
   uint64_t wait_ns;
 };
 
 struct ExpandShared {
   Tile tile;
+  Adapter group[XN];   // what this CTA adds or copies, in turn
   uint64_t t_full, full[2], empty[2], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
@@ -274,18 +287,14 @@ __device__ __forceinline__ Channels channels_of(const ExpandArgs& p, int tile) {
   return c;
 }
 
-// barrier of 128 epilogue threads; the second says whether `ok` holds in all of them
-__device__ __forceinline__ void half_bar(int half) {
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-}
-__device__ __forceinline__ bool half_all(int half, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r)
-      : "r"((uint32_t)ok), "r"(1 + half)
-      : "memory");
-  return r != 0;
+// An item of expand's work: one adapter of the block and a channel tile.  The CTA
+// of index c takes items c, c + step, ... of all of them, adapter by adapter.
+struct Item {
+  int g, tile;
+};
+__device__ __forceinline__ Item next_item(const ExpandArgs& p, Item it) {
+  for (it.tile += p.step; it.tile >= p.tiles; it.tile -= p.tiles) ++it.g;
+  return it;
 }
 
 __global__ void __launch_bounds__(X_THREADS, 2)
@@ -294,9 +303,10 @@ __global__ void __launch_bounds__(X_THREADS, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ ExpandShared sh;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // every block's first adapter before any block's second
-  const int per_slot = p.blocks * p.step, slot = blockIdx.x / per_slot, at_slot = blockIdx.x - slot * per_slot;
-  const int block = at_slot / p.step, tile0 = at_slot - block * p.step, row0 = block * XN;
+  if (warp == 1) tmem_take(&sh.tmem, 2 * XN);
+  const int block = blockIdx.x / p.step, row0 = block * XN;
+  const int index = blockIdx.x - block * p.step;
+  const Item first = {index / p.tiles, index % p.tiles};
   if (warp == 0 && elect_one()) {
     prefetch_tmap(&bmap);
     prefetch_tmap(&tmap);
@@ -311,221 +321,235 @@ __global__ void __launch_bounds__(X_THREADS, 2)
     sh.abort = 0;
     fence_barrier_init();
   }
+  tc_fence_before();
   pdl_trigger();
   group_rows(p.l, sh.tile, row0, XN, false, p.l.out != p.l.y);
-  if (__popcll(sh.tile.leads) <= slot) {   // nothing for this CTA
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int groups = __popcll(sh.tile.leads);
+  if (groups <= first.g) {   // nothing for this CTA
+    if (warp == 1) tmem_give(tmem, 2 * XN);
     pdl_wait();
     return;
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(2 * XN));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if (threadIdx.x < XN && (sh.tile.leads >> threadIdx.x & 1)) {
+    const int i = __popcll(sh.tile.leads & ((1ull << threadIdx.x) - 1)), id = sh.tile.id[threadIdx.x];
+    sh.group[i] = id >= 0 ? adapter_of(p.l, sh.tile, id) : Adapter{id, 0, 0.f};
   }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem;
   const int b_bytes = p.kb * B_TILE;
   uint8_t *b_smem = smem, *t_smem = smem + 2 * b_bytes;   // t: [slice][kb][hi, lo]
   float* stg = reinterpret_cast<float*>(t_smem + p.l.S * p.kb * 2 * T_TILE);
   int buf = 0, issued = 0;     // ring position = accumulator: one B tile per output tile
   uint32_t phase = 0;
-  bool ok = true, have_t = false;
+  bool ok = true;
 
-  unsigned long long leads = sh.tile.leads;
-  for (int gi = 0; leads && ok; ++gi, leads &= leads - 1) {
-    if (gi % p.l.slots != slot) continue;
-    const int id = sh.tile.id[__ffsll((long long)leads) - 1];
-    Adapter ad = {};
-    if (id >= 0) ad = adapter_of(p.l, sh.tile, id);
-    const int steps = (ad.ra + 15) / 16;   // of 16 ranks; 0: rows are copied
-    if (warp == 0) {
-      const int kb = (steps + 3) / 4;
-      for (int tile = tile0; steps > 0 && tile < p.tiles; tile += p.step) {
-        ok = warp_wait(&sh.empty[buf], phase ^ 1, p.wait_ns);
-        if (!ok) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&sh.full[buf], kb * B_TILE);
-          for (int i = 0; i < kb; ++i)
-            tma_load_2d(b_smem + buf * b_bytes + i * B_TILE, &bmap, &sh.full[buf], i * BKE,
-                        id * p.l.N + channels_of(p, tile).lo);
-        }
-        __syncwarp();
-        if (!have_t) {   // every slice's t of these rows, once; the first read that waits for shrink
-          pdl_wait();
-          if (elect_one()) {
-            mbar_arrive_expect_tx(&sh.t_full, p.l.S * p.kb * 2 * T_TILE);
-            for (int i = 0; i < p.l.S * p.kb; ++i) {
-              uint8_t* t = t_smem + i * 2 * T_TILE;
-              tma_load_2d(t, &tmap, &sh.t_full, i * BKE, row0);
-              tma_load_2d(t + T_TILE, &tmap, &sh.t_full, p.ld_t + i * BKE, row0);
-            }
-          }
-          __syncwarp();
-          have_t = true;
-        }
-        ++issued;
-        phase ^= buf;
-        buf ^= 1;
+  // every warp goes through the same items, group by group and tile by tile,
+  // without a barrier between groups
+  if (warp == 0) {
+    for (Item it = first; it.g < groups; it = next_item(p, it)) {
+      const Adapter ad = sh.group[it.g];
+      if (ad.ra == 0) continue;
+      ok = warp_wait(&sh.empty[buf], phase ^ 1, p.wait_ns);
+      if (!ok) break;
+      if (elect_one()) {
+        const int kb = (ad.ra + BKE - 1) / BKE;
+        mbar_arrive_expect_tx(&sh.full[buf], kb * B_TILE);
+        for (int i = 0; i < kb; ++i)
+          tma_load_2d(b_smem + buf * b_bytes + i * B_TILE, &bmap, &sh.full[buf], i * BKE,
+                      ad.id * p.l.N + channels_of(p, it.tile).lo);
       }
-    } else if (warp == 1) {
-      for (int tile = tile0; steps > 0 && tile < p.tiles; tile += p.step) {
-        ok = warp_wait(&sh.tempty[buf], phase ^ 1, p.wait_ns) && warp_wait(&sh.full[buf], phase, p.wait_ns) &&
-             warp_wait(&sh.t_full, 0, p.wait_ns);
-        if (!ok) break;
-        uint8_t* bs = b_smem + buf * b_bytes;
-        if (ad.ra & 15) {
-          // the last step's ranks past the adapter's: B's columns there are not
-          // part of it, whatever they hold
-          const int from = ad.ra & 63, to = ((ad.ra + 15) & ~15) - (ad.ra & ~63);
-          uint8_t* b = bs + (ad.ra / 64) * B_TILE;
-          for (int row = lane; row < TILE_J; row += 32)
-            for (int c = from; c < to; ++c)
-              *reinterpret_cast<uint16_t*>(b + row * 128 + (((c >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0;
-          fence_proxy_async();
-        }
-        __syncwarp();
+      __syncwarp();
+      if (issued == 0) {   // every slice's t of these rows, once; the first read that waits for shrink
+        pdl_wait();
         if (elect_one()) {
-          tc_fence_after();
-          const uint32_t idesc =
-              (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XN >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
-          const uint64_t b0 = sdesc_sw128(smem_u32(bs));
-          const uint64_t t0 = sdesc_sw128(smem_u32(t_smem + channels_of(p, tile).sl * p.kb * 2 * T_TILE));
-          for (int i = 0; i < steps; ++i) {
-            const uint64_t b = b0 + (uint32_t)((i >> 2) * B_TILE >> 4) + (i & 3) * 2;
-            const uint64_t t = t0 + (uint32_t)((i >> 2) * 2 * T_TILE >> 4) + (i & 3) * 2;
-            umma_bf16(tmem + buf * XN, b, t + (T_TILE >> 4), idesc, i != 0);   // lo
-            umma_bf16(tmem + buf * XN, b, t, idesc, 1);                        // hi
+          mbar_arrive_expect_tx(&sh.t_full, p.l.S * p.kb * 2 * T_TILE);
+          for (int i = 0; i < p.l.S * p.kb; ++i) {
+            uint8_t* t = t_smem + i * 2 * T_TILE;
+            tma_load_2d(t, &tmap, &sh.t_full, i * BKE, row0);
+            tma_load_2d(t + T_TILE, &tmap, &sh.t_full, p.ld_t + i * BKE, row0);
           }
-          umma_commit(&sh.empty[buf]);
-          umma_commit(&sh.tfull[buf]);
         }
         __syncwarp();
-        ++issued;
-        phase ^= buf;
-        buf ^= 1;
       }
-    } else {
-      // two groups of 128 threads, 32 token rows each.  A thread takes eight
-      // channels of every eighth row: 16 lanes access 256 contiguous bytes
-      const int half = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127, g8 = (et & 15) * 8, tr = half * 32 + (et >> 4);
-      const int quarter = warp & 3;   // the TMEM lanes this warp may read
-      float* mine = stg + half * 16 * TILE_J;
-      bool rows[4];
+      ++issued;
+      phase ^= buf;
+      buf ^= 1;
+    }
+  } else if (warp == 1) {
+    for (Item it = first; it.g < groups; it = next_item(p, it)) {
+      const Adapter ad = sh.group[it.g];
+      const int steps = (ad.ra + 15) / 16;   // of 16 ranks
+      if (steps == 0) continue;
+      ok = warp_wait(&sh.tempty[buf], phase ^ 1, p.wait_ns) && warp_wait(&sh.full[buf], phase, p.wait_ns) &&
+           warp_wait(&sh.t_full, 0, p.wait_ns);
+      if (!ok) break;
+      uint8_t* bs = b_smem + buf * b_bytes;
+      if (ad.ra & 15) {
+        // the last step's ranks past the adapter's: B's columns there are not
+        // part of it, whatever they hold
+        const int from = ad.ra & 63, to = ((ad.ra + 15) & ~15) - (ad.ra & ~63);
+        uint8_t* b = bs + (ad.ra / 64) * B_TILE;
+        for (int row = lane; row < TILE_J; row += 32)
+          for (int c = from; c < to; ++c)
+            *reinterpret_cast<uint16_t*>(b + row * 128 + (((c >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0;
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (elect_one()) {
+        tc_fence_after();
+        const uint32_t idesc =
+            (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XN >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
+        const uint64_t b0 = sdesc_sw128(smem_u32(bs));
+        const uint64_t t0 = sdesc_sw128(smem_u32(t_smem + channels_of(p, it.tile).sl * p.kb * 2 * T_TILE));
+        for (int i = 0; i < steps; ++i) {
+          const uint64_t b = b0 + (uint32_t)((i >> 2) * B_TILE >> 4) + (i & 3) * 2;
+          const uint64_t t = t0 + (uint32_t)((i >> 2) * 2 * T_TILE >> 4) + (i & 3) * 2;
+          umma_bf16(tmem + buf * XN, b, t + (T_TILE >> 4), idesc, i != 0);   // lo
+          umma_bf16(tmem + buf * XN, b, t, idesc, 1);                        // hi
+        }
+        umma_commit(&sh.empty[buf]);
+        umma_commit(&sh.tfull[buf]);
+      }
+      __syncwarp();
+      ++issued;
+      phase ^= buf;
+      buf ^= 1;
+    }
+  } else {
+    // A warp takes 32 channels (its lanes of TMEM) of 32 token rows, a thread
+    // eight channels of every eighth row, so a warp accesses rows in runs of 64
+    // bytes.  It transposes 16 rows at a time through staging of its own: with
+    // 128 threads on one staging area and a branch per row an item took twice as long.
+    const int half = (warp - 2) >> 2, quarter = warp & 3;
+    const int tr = half * 32 + (lane >> 2), j0 = quarter * 32 + (lane & 3) * 8;
+    float* to = stg + (warp - 2) * 16 * X_LD + lane;
+    const float* from = stg + (warp - 2) * 16 * X_LD + (lane >> 2) * X_LD + (lane & 3) * 8;
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const int row_id = sh.tile.id[half * 32 + lane];
+    struct Part {   // an item's part of this warp
+      int id, lo;
+      bool whole, in;   // all 32 x 32 outputs, any of this thread's channels
+    };
+    auto part_of = [&](Item it) {
+      const Channels c = channels_of(p, it.tile);
+      Part w;
+      w.id = sh.group[it.g].id;
+      w.lo = c.lo;
+      w.in = c.lo + j0 < c.end;
+      w.whole = __all_sync(0xffffffffu, row_id == w.id && w.in);
+      return w;
+    };
+    auto load_y = [&](Item it, uint4 (&y)[4]) {
+      if (it.g >= groups) return;
+      const Part w = part_of(it);
+      const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + w.lo + j0;
+      if (w.whole) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rows[i] = sh.tile.id[tr + i * 8] == id;
-      auto load_y = [&](int tile, uint4 (&y)[4]) {
-        if (tile >= p.tiles) return;
-        const Channels c = channels_of(p, tile);
-        const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + c.lo + g8;
+        for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
+      } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (c.lo + g8 < c.end && rows[i]) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
-      };
-      // a tile further ahead: its lines into L2, one per thread
-      const int pr = half * 32 + (et >> 2), pc = (et & 1) * 64;
-      const bool p_row = (et & 2) == 0 && sh.tile.id[pr] == id;
-      auto prefetch_y = [&](int tile) {
-        if (tile >= p.tiles || !p_row) return;
-        const Channels c = channels_of(p, tile);
-        if (c.lo + pc < c.end)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.l.y + (int64_t)(row0 + pr) * p.l.ldy + c.lo + pc));
-      };
-      auto finish = [&](int tile, const uint4 (&y)[4]) {
-        const Channels ch = channels_of(p, tile);
-        const bool in = ch.lo + g8 < ch.end;
-        if (steps > 0) {
-          // 128 threads go on together or not at all
-          ok = mbar_wait(&sh.tfull[buf], phase, p.wait_ns);
-          if (!ok) {
-            atomicExch(p.l.status, TSDS_E_TIMEOUT);
-            *(volatile int*)&sh.abort = 1;
-          }
-          __syncwarp();
-          ok = half_all(half, ok);
-          if (!ok) return;
-          tc_fence_after();
-        }
-        bf16* to_out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + ch.lo + g8;
+          if (w.in && sh.tile.id[tr + i * 8] == w.id) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
+      }
+    };
+    // an item further ahead: its lines into L2, one per thread of every other warp
+    auto prefetch_y = [&](Item it) {
+      if (it.g >= groups || (quarter & 1) || row_id != sh.group[it.g].id) return;
+      const Channels c = channels_of(p, it.tile);
+      if (c.lo + quarter * 32 < c.end)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.l.y + (int64_t)(row0 + half * 32 + lane) * p.l.ldy + c.lo +
+                                                      quarter * 32));
+    };
+    auto finish = [&](Item it, const uint4 (&y)[4]) {
+      const Part w = part_of(it);
+      bf16* out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + w.lo + j0;
+      if (sh.group[it.g].ra == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (w.in && sh.tile.id[tr + i * 8] == w.id) *reinterpret_cast<uint4*>(out + i * 8 * p.l.ldo) = y[i];
+        return;
+      }
+      ok = warp_wait(&sh.tfull[buf], phase, p.wait_ns);
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t v[32];
+      tmem_request32(tmem + buf * XN + ((uint32_t)(quarter * 32) << 16) + half * 32, v);
+      tmem_wait32(v);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.tempty[buf]);   // this warp has read its part of the accumulator
+      auto rest = [&](auto whole) {
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {
-          if (steps > 0) {
-            float v[16];
-            tmem_ld16(tmem + buf * XN + ((uint32_t)(quarter * 32) << 16) + half * 32 + c, v);
-            float* to = mine + quarter * 32 + lane;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[i * TILE_J] = v[i];
-            if (c == 16) {   // the accumulator is read
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh.tempty[buf]);
-            }
-            half_bar(half);
-          }
+          for (int i = 0; i < 16; ++i) to[i * X_LD] = __uint_as_float(v[c + i]);
+          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int k = c / 8 + i;
-            if (in && rows[k]) {
-              uint4 o = y[k];
-              if (steps > 0) {
-                const float4* d = reinterpret_cast<const float4*>(mine + ((et >> 4) + i * 8) * TILE_J + g8);
-                const float4 a = d[0], b = d[1];
-                o = make_uint4(pack_bf2(bf_lo(o.x) + a.x, bf_hi(o.x) + a.y), pack_bf2(bf_lo(o.y) + a.z, bf_hi(o.y) + a.w),
-                               pack_bf2(bf_lo(o.z) + b.x, bf_hi(o.z) + b.y), pack_bf2(bf_lo(o.w) + b.z, bf_hi(o.w) + b.w));
-              }
-              *reinterpret_cast<uint4*>(to_out + k * 8 * p.l.ldo) = o;
-            }
+            const float4 a = *reinterpret_cast<const float4*>(from + i * 8 * X_LD);
+            const float4 b = *reinterpret_cast<const float4*>(from + i * 8 * X_LD + 4);
+            const uint4 o = y[k];
+            if (whole || (w.in && sh.tile.id[tr + k * 8] == w.id))
+              *reinterpret_cast<uint4*>(out + k * 8 * p.l.ldo) = make_uint4(
+                  pack_bf2(bf_lo(o.x) + a.x, bf_hi(o.x) + a.y), pack_bf2(bf_lo(o.y) + a.z, bf_hi(o.y) + a.w),
+                  pack_bf2(bf_lo(o.z) + b.x, bf_hi(o.z) + b.y), pack_bf2(bf_lo(o.w) + b.z, bf_hi(o.w) + b.w));
           }
           __syncwarp();
-          if (steps > 0) half_bar(half);   // the staging area is free
-        }
-        if (steps > 0) {
-          phase ^= buf;
-          buf ^= 1;
         }
       };
-      // the next tile's y is requested before this one's is used, in a register
-      // set of its own: loads are awaited by set, so one set would be awaited
-      // with the requests just made (5 us a tile instead of 1.2)
-      uint4 y0[4], y1[4];
-      load_y(tile0, y0);
-      prefetch_y(tile0 + p.step);
-      prefetch_y(tile0 + 2 * p.step);
-      if (steps == 0) pdl_wait();
-      for (int tile = tile0; ok && tile < p.tiles; tile += 2 * p.step) {
-        load_y(tile + p.step, y1);
-        prefetch_y(tile + 3 * p.step);
-        finish(tile, y0);
-        if (!ok || tile + p.step >= p.tiles) break;
-        load_y(tile + 2 * p.step, y0);
-        prefetch_y(tile + 4 * p.step);
-        finish(tile + p.step, y1);
-      }
+      if (w.whole)
+        rest(Yes());
+      else
+        rest(No());
+      phase ^= buf;
+      buf ^= 1;
+    };
+    // the next item's y is requested before this one's is used, in a register
+    // set of its own: loads are awaited by set, so one set would be awaited
+    // with the requests just made (5 us a tile instead of 1.2)
+    uint4 y0[4], y1[4];
+    Item now = first, next = next_item(p, now), ahead = next_item(p, next);
+    load_y(now, y0);
+    prefetch_y(next);
+    prefetch_y(ahead);
+    pdl_wait();   // a copied row may be what an earlier kernel still reads
+    while (now.g < groups) {
+      ahead = next_item(p, ahead);
+      load_y(next, y1);
+      prefetch_y(ahead);
+      finish(now, y0);
+      if (!ok || next.g >= groups) break;
+      now = next_item(p, next);
+      ahead = next_item(p, ahead);
+      load_y(now, y0);
+      prefetch_y(ahead);
+      finish(next, y1);
+      if (!ok) break;
+      next = next_item(p, now);
     }
-    if (warp < 2 && !ok) {
-      if (lane == 0) atomicExch(p.l.status, TSDS_E_TIMEOUT);
-      *(volatile int*)&sh.abort = 1;
-    }
-    __syncwarp();
-    __syncthreads();
-    ok = !*(volatile int*)&sh.abort;
-    __syncthreads();
   }
+  if (!ok) {
+    if (lane == 0) atomicExch(p.l.status, TSDS_E_TIMEOUT);
+    *(volatile int*)&sh.abort = 1;
+  }
+  __syncwarp();
   pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (sh.abort) {   // uniform: copies and MMAs in flight finish (bounded) before TMEM is freed
     if (warp == 0 && lane == 0) {
       drain_tma_ring(sh.full, 2, issued);
-      if (have_t) mbar_wait(&sh.t_full, 0, 20000000ull);
+      if (issued > 0) mbar_wait(&sh.t_full, 0, 20000000ull);   // requested behind the first tile
     }
     if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
     __syncthreads();
   }
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * XN));
+    tmem_give(tmem, 2 * XN);
   }
 }
 
@@ -569,17 +593,14 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.tmem_cols = p.nt;
   p.idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.nt >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
   p.wait_ns = tsds_get_wait_limit_ns();
-  // A cluster (CTA) per adapter of a block of rows as long as all are resident at
+  // A cluster per adapter of a block of rows as long as all are resident at
   // once; beyond that each takes several in turn.  One without an adapter
   // holds the next launch up: with twice as many the q/k/v adapters of 2048
   // rows take 61 us instead of 48.
-  auto slots_of = [&](int blocks, int rows, int most) {
-    int n = most / blocks;
-    n = n < 1 ? 1 : (n > rows ? rows : n);
-    return n > l.n_adapters + 1 ? l.n_adapters + 1 : n;
-  };
   const int sms = tsds_tc_num_sms();
-  p.l.slots = slots_of(p.blocks, p.nt, 2 * sms / CL);
+  p.l.slots = 2 * sms / CL / p.blocks;
+  p.l.slots = p.l.slots < 1 ? 1 : (p.l.slots > p.nt ? p.nt : p.l.slots);
+  if (p.l.slots > l.n_adapters) p.l.slots = l.n_adapters;
   CUtensorMap a_all, a_box, xmap, bmap, tmap;
   const uint64_t a_rows = (uint64_t)l.n_adapters * SR;
   int st = tsds_make_tmap_2d_bf16(&a_all, l.a, l.K, a_rows, (uint64_t)l.K * 2, BKE, p.arows, 1);
@@ -605,15 +626,14 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   q.tiles = q.first_tile[l.S];
   q.wait_ns = p.wait_ns;
   const int smem = 2 * q.kb * B_TILE + l.S * q.kb * 2 * T_TILE + X_STAGING + 1024;
-  // channel tiles of a block over as many CTAs as are resident at once
-  const int places = sms * (smem <= 112 * 1024 ? 2 : 1);
+  // a block's items over as many CTAs as are resident at once
+  const int places = sms * (smem <= 112 * 1024 ? 2 : 1), most = q.tiles * (l.n_adapters < XN ? l.n_adapters + 1 : XN);
   q.step = places / q.blocks;
-  q.step = q.step < 1 ? 1 : (q.step > q.tiles ? q.tiles : q.step);
-  q.l.slots = slots_of(q.blocks * q.step, XN, places);
+  q.step = q.step < 1 ? 1 : (q.step > most ? most : q.step);
   static tsds_device_flags expand_set;
   st = tsds_smem_limit_once(expand_kernel, 220 * 1024, expand_set);
   if (st != TSDS_OK) return st;
-  tsds_launch(expand_kernel, dim3((unsigned)(q.blocks * q.step * q.l.slots)), dim3(X_THREADS), smem, stream, bmap, tmap,
+  tsds_launch(expand_kernel, dim3((unsigned)(q.blocks * q.step)), dim3(X_THREADS), smem, stream, bmap, tmap,
               q);
   return tsds_launch_status();
 }
