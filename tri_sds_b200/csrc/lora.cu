@@ -35,13 +35,26 @@ using namespace tsds::lora;
 
 namespace {
 
-// Whether one launch of this file's kernel runs, or the two of lora_tc.cu: by
-// the rows, which this kernel takes 16 at a time, and the size of t.  Measured
-// (K 5120, outputs 10240 in three slices or 8192 -> 5120 in one): 512 rows at
-// rank 16 (t of 25 K elements) 17 us here, 25 there; 768 rows (37 K) 27 and 28;
-// 208 rows at rank 64 (40 K) 36 and 33; 1024 rows at rank 16 in one slice (16 K) 25
-// and 29, at rank 64 (66 K) 36 and 30; 2048 rows at rank 8 (16 K) 48 and 39.
-bool few_rows(int M, int R, int S) { return M <= 1024 && (int64_t)M * S * R <= 36864; }
+constexpr int CL = 8;         // CTAs per cluster
+constexpr int TR = 16;        // rows per tile: one m16 tile
+constexpr int RANKS = 64;     // columns of t, at most: 8 n8 tiles
+
+// Whether one launch of this file's kernel runs, or the two of lora_tc.cu.  A
+// cluster here reads all ranks of every slice for 16 rows, so the columns of t,
+// the rows' bytes and the (tile, adapter) pairs decide; how many pairs occur is known
+// only up to tiles x min(adapters, 16).  Measured, here and there (K 5120 into
+// q/k/v of 10240, or K 8192 -> 5120): 8 rows of 8 adapters, rank 16 in three slices
+// 10.9 and 15.0 us, rank 32 in three 16.7 and 15.6, rank 64 in one 13.6 and 15.2; 32
+// rows, rank 64 in one 13.3 and 12.5; 8 x 26 rows, rank 16 in three 14.3 and 15.8, rank
+// 32 in three 22.4 and 16.6; 512 rows of one adapter, rank 16 in three 15.1 and 16.8,
+// rank 16 in one 12.5 and 15.0, 1024 rows 23.6 and 18.4; 128 rows that alternate
+// between 16 adapters, rank 16 in one 45 and 28.  K 25600 -> 5120: 512 rows, rank
+// 64 43 and 22.8; 208 rows, rank 16 19.3 and 20.9.
+bool few_rows(int M, int K, int R, int S, int n_adapters) {
+  const int tiles = (M + TR - 1) / TR, SR = S * R;
+  if (M > 512 || tiles * (n_adapters < TR ? n_adapters : TR) > 104) return false;
+  return SR <= 16 || (SR <= 48 && (int64_t)tiles * K <= 200000) || (SR <= RANKS && M <= TR);
+}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -59,9 +72,6 @@ __device__ __forceinline__ uint4 ld16(const bf16* p) { return *reinterpret_cast<
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
-
-constexpr int CL = 8;    // CTAs per cluster
-constexpr int TR = 16;   // rows per tile: one m16 tile
 
 // The adapter at hand, and its layout: n8 tiles and chunks of 16 of a slice's
 // ranks, columns of t per slice.
@@ -104,11 +114,11 @@ __device__ __forceinline__ void prefetch_second(const LoraArgs& p, const Tile& s
   }
 }
 
-// t's columns for rank tiles t0 .. t0 + nt - 1: the cluster's partial sums
-// (part: [TR][ldr] in every CTA) of this CTA's share of the rows, scaled, as
-// two bf16 words into every CTA's t_hi / t_lo.
+// t's columns (nt rank tiles): the cluster's partial sums (part: [TR][ldr] in
+// every CTA) of this CTA's share of the rows, scaled, as two bf16 words into
+// every CTA's t_hi / t_lo.
 __device__ __forceinline__ void exchange(const LoraArgs& p, const Ranks& ad, float* part, int ldr, bf16* t_hi,
-                                         bf16* t_lo, int t0, int nt, int rank) {
+                                         bf16* t_lo, int nt, int rank) {
   tc::cluster_barrier();   // every CTA's part is complete
   constexpr int SHARE = TR / CL;
   const int n4 = nt * 2;
@@ -121,7 +131,7 @@ __device__ __forceinline__ void exchange(const LoraArgs& p, const Ranks& ad, flo
     float4 s = f[0];
 #pragma unroll
     for (int k = 1; k < CL; ++k) s = make_float4(s.x + f[k].x, s.y + f[k].y, s.z + f[k].z, s.w + f[k].w);
-    const int ti = t0 + c4 / 2, sl = ti / ad.nr8;
+    const int ti = c4 / 2, sl = ti / ad.nr8;
     const int to = m * p.ld_t + sl * ad.Rp + (ti - sl * ad.nr8) * 8 + (c4 & 1) * 4;
     const float v[4] = {s.x * ad.scale, s.y * ad.scale, s.z * ad.scale, s.w * ad.scale};
     float h[4];
@@ -219,16 +229,16 @@ __device__ __forceinline__ void expand(const LoraArgs& p, const Tile& sh, const 
   }
 }
 
-// The first product.  NT: n8 rank tiles per pass over K, U: chunks of 32 k loaded
+// The first product.  NT: most n8 rank tiles, U: chunks of 32 k loaded
 // together, PER_SM: CTAs per SM.
 template <int NT, int U, int WARPS, int PER_SM>
 struct First {
-  static constexpr int CTAS = PER_SM, THREADS = WARPS * 32, PASS = NT, LDR = NT * 8 + 4;   // LDR: padded row of partial sums
+  static constexpr int CTAS = PER_SM, THREADS = WARPS * 32, LDR = NT * 8 + 4;   // LDR: padded row of partial sums
   static constexpr int PART = WARPS * TR * LDR * (int)sizeof(float);   // the CTA's sum, behind those of its warps
   static constexpr int WORK = PART + TR * LDR * (int)sizeof(float);
 
   static __device__ __forceinline__ void run(const LoraArgs& p, const Ranks& ad, uint8_t* work, float* part, int row0,
-                                             int rank, int t0, int nt) {
+                                             int rank, int nt) {
     float* red = reinterpret_cast<float*>(work);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
     const bf16* a_id = p.a + (int64_t)ad.id * p.S * p.R * p.K + 8 * q;
@@ -236,7 +246,7 @@ struct First {
     int ar[NT];   // rank row of each tile, -1: none
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int s = (t0 + i) / ad.nr8, r = (t0 + i - s * ad.nr8) * 8 + g;
+      const int s = i / ad.nr8, r = (i - s * ad.nr8) * 8 + g;
       ar[i] = i < nt && r < ad.ra ? s * p.R + r : -1;
     }
     float acc[NT][4];
@@ -251,7 +261,7 @@ struct First {
       // that only the first round waits for DRAM
       const uint32_t bytes = (uint32_t)(hi - lo) * 64;
       for (int i = tid; i < nt * 8 + TR; i += THREADS) {
-        const int u = t0 + i / 8, s = u / ad.nr8, r = (u - s * ad.nr8) * 8 + i % 8, m = row0 + i - nt * 8;
+        const int u = i / 8, s = u / ad.nr8, r = (u - s * ad.nr8) * 8 + i % 8, m = row0 + i - nt * 8;
         if (i < nt * 8 && r < ad.ra)
           prefetch_l2(p.a + ((int64_t)ad.id * p.S * p.R + s * p.R + r) * p.K + lo * 32, bytes);
         else if (i >= nt * 8 && m < p.M)
@@ -335,11 +345,10 @@ __global__ void __launch_bounds__(F::THREADS, F::CTAS) lora_kernel(LoraArgs p) {
     ad.nch = (ad.ra + 15) / 16;
     ad.Rp = (p.R + 15) / 16 * 16;
     prefetch_second(p, sh, ad, row0, rank);
-    const int tiles8 = p.S * ad.nr8;
-    for (int t0 = 0; t0 < tiles8; t0 += F::PASS) {
-      const int nt = tiles8 - t0 < F::PASS ? tiles8 - t0 : F::PASS;
-      F::run(p, ad, dyn, part, row0, rank, t0, nt);
-      exchange(p, ad, part, F::LDR, t_hi, t_lo, t0, nt, rank);
+    const int nt = p.S * ad.nr8;
+    if (nt > 0) {
+      F::run(p, ad, dyn, part, row0, rank, nt);
+      exchange(p, ad, part, F::LDR, t_hi, t_lo, nt, rank);
     }
     // an odd number of rank tiles: the last chunk of 16 ends in zeros
     if (ad.nr8 & 1) {
@@ -361,7 +370,7 @@ template <typename F>
 int launch_lora(LoraArgs p, cudaStream_t stream) {
   static tsds_device_flags limit_set;
   const int smem = F::WORK + 2 * TR * p.ld_t * (int)sizeof(bf16);
-  constexpr int most = F::WORK + 2 * TR * (MAX_SLICES * MAX_RANK + 16) * (int)sizeof(bf16);
+  constexpr int most = F::WORK + 2 * TR * (RANKS + 16) * (int)sizeof(bf16);
   static_assert(most <= 226 * 1024, "shared memory of a CTA");
   const int st = tsds_smem_limit_once(lora_kernel<F>, most, limit_set);
   if (st != TSDS_OK) return st;
@@ -379,7 +388,8 @@ int launch_lora(LoraArgs p, cudaStream_t stream) {
 }  // namespace
 
 extern "C" size_t tsds_lora_workspace_bytes(int M, int R, int n_slices) {
-  if (M <= 0 || R <= 0 || n_slices <= 0 || few_rows(M, R, n_slices)) return 0;
+  // whatever K and the number of adapters are
+  if (M <= 0 || R <= 0 || n_slices <= 0 || (M <= TR && n_slices * R <= RANKS)) return 0;
   return tsds_lora_tc_workspace_bytes(M, R, n_slices);
 }
 
@@ -432,15 +442,15 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   // rows of t: 16 elements past a multiple of 64, so that the fragments'
   // 8-byte reads of four rows cover all banks
   p.ld_t = (n_slices * ((R + 15) / 16 * 16) + 63) / 64 * 64 + 16;
-  if (!few_rows(M, R, n_slices)) {
+  if (!few_rows(M, K, R, n_slices, n_adapters)) {
     TSDS_RETURN_IF(!workspace || workspace_bytes < tsds_lora_tc_workspace_bytes(M, R, n_slices), TSDS_E_WORKSPACE);
     TSDS_RETURN_IF(!tsds_aligned16(workspace), TSDS_E_ALIGN);
     return tsds_lora_tc(p, workspace, stream);
   }
   // Where a cluster for every adapter of every tile fits the SMs at once the call
   // is a matter of latency: many warps and loads per CTA (q/k/v adapters of 8
-  // one-token requests 11.2 us, 14.2 with the smaller CTAs).  With more of them two
-  // smaller CTAs per SM overlap (8 x 26 rows 14.4 us, 21.7 with the larger ones).
+  // one-token requests 10.9 us, 14.2 with the smaller CTAs).  With more of them two
+  // smaller CTAs per SM overlap (8 x 26 rows 14.3 us, 21.7 with the larger ones).
   const int most = (M + TR - 1) / TR * (n_adapters < TR ? n_adapters : TR);
   if (most > tsds_tc_num_sms() / CL) return launch_lora<First<8, 1, 8, 2>>(p, stream);
   if (n_slices * R <= 16) return launch_lora<First<2, 4, 16, 1>>(p, stream);

@@ -8,13 +8,17 @@
 //   through a TMA ring.  The partial sums meet over distributed shared memory
 //   (rank order: always the same bits), and t is stored as two bf16 words
 //   (hi + lo, 16 bits of it), so its rounding is far below the output's.
-// * expand: out = y + B t^T, one CTA per 128 output channels x 64 token rows
-//   x adapter, several CTAs per SM: its y is requested while shrink still runs,
-//   the products of both words of t go into one TMEM accumulator, and the
-//   epilogue stores whole lines.
+// * expand: out = y + B t^T.  An item is 128 output channels x 64 token rows x
+//   adapter; two CTAs per SM share a block's items and take theirs in one
+//   sequence, with B and y of the next items on their way.  The products of
+//   both words of t go into one TMEM accumulator, two of which alternate, and
+//   each epilogue warp adds its 32 channels of 32 rows to y by itself.
 //
 // The bytes of x and y bound both (B and A come from L2 after their first
-// use); the MMAs are a few percent of the tensor cores' rate.
+// use); the MMAs are a few percent of the tensor cores' rate.  2048 rows, K 5120,
+// rank 32 into q/k/v of 10240 columns: 36 us, shrink about 13 of them (21 MB of x, the
+// rest the chain from launch to reduction) and expand 21 (84 MB of y and out,
+// 4 TB/s).  Asking for y from shrink already, into L2, made it 43.
 // shrink lets its successor start only after its own dependency wait, so
 // everything before shrink is complete when expand begins, and expand may
 // read y, B and the indices before its wait; only t comes after it.
@@ -580,8 +584,10 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.t = (bf16*)workspace;
   p.Rp = rank_columns(l.R);
   p.ld_t = l.S * p.Rp;
-  // token rows per shrink block: 32 for a few hundred rows (more clusters), 64 above
-  p.nt = l.M <= 512 ? 32 : 64;
+  // Token rows per shrink block: 32 for few rows (more clusters; 8 x 26 rows at
+  // rank 64 into q/k/v 23.7 us, with 64 26.6), 64 above (an adapter's A is read
+  // less often; 16 x 26 rows, K 25600, rank 16 25.0 us, with 32 37.7)
+  p.nt = l.M <= 256 ? 32 : 64;
   p.blocks = (l.M + p.nt - 1) / p.nt;
   const int SR = l.S * l.R;
   p.arows = SR < TILE_J ? SR : TILE_J;
@@ -595,8 +601,8 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.wait_ns = tsds_get_wait_limit_ns();
   // A cluster per adapter of a block of rows as long as all are resident at
   // once; beyond that each takes several in turn.  One without an adapter
-  // holds the next launch up: with twice as many the q/k/v adapters of 2048
-  // rows take 61 us instead of 48.
+  // holds the next launch up: with twice as many the q/k/v adapters of 256 rows
+  // that alternate between 8 adapters of rank 64 take 47 us instead of 44.
   const int sms = tsds_tc_num_sms();
   p.l.slots = 2 * sms / CL / p.blocks;
   p.l.slots = p.l.slots < 1 ? 1 : (p.l.slots > p.nt ? p.nt : p.l.slots);
