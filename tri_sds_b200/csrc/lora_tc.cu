@@ -125,12 +125,11 @@ __global__ void __launch_bounds__(THREADS)
       const bool all = ad.ra == p.l.R;
       if (warp == 0 && alive) {
         // small boxes of this pass: only the ranks that the adapter uses
-        int bytes = p.nt * 128 + p.arows * 128;
-        if (!all) {
-          bytes = p.nt * 128;
-          for (int u = u0; u < u0 + p.arows && u < p.l.S * p.l.R; u += p.bx)
-            if (u % p.l.R < ad.ra) bytes += p.bx * 128;
-        }
+        uint32_t boxes = 0;
+        if (!all)
+          for (int i = 0, u = u0; u < u0 + p.arows && u < p.l.S * p.l.R; ++i, u += p.bx)
+            if (u % p.l.R < ad.ra) boxes |= 1u << i;
+        const int bytes = p.nt * 128 + (all ? p.arows : __popc(boxes) * p.bx) * 128;
         for (int i = 0; i < nk; ++i) {
           alive = warp_wait(&sh.empty[s], phase, p.wait_ns);
           if (!alive) break;
@@ -142,8 +141,10 @@ __global__ void __launch_bounds__(THREADS)
             if (all) {
               tma_load_2d(a, &a_all, &sh.full[s], k, a_row + u0);
             } else {
-              for (int u = u0; u < u0 + p.arows && u < p.l.S * p.l.R; u += p.bx)
-                if (u % p.l.R < ad.ra) tma_load_2d(a + (u - u0) * 128, &a_box, &sh.full[s], k, a_row + u);
+              for (uint32_t b = boxes; b; b &= b - 1) {
+                const int u = (__ffs(b) - 1) * p.bx;
+                tma_load_2d(a + u * 128, &a_box, &sh.full[s], k, a_row + u0 + u);
+              }
             }
           }
           __syncwarp();
