@@ -41,6 +41,19 @@ def test_quant(ops, rows, n):
     ref.check_quant(q, s, x.double(), 2 * ref.F32)
 
 
+@pytest.mark.parametrize("n", [8208, 9024, 16384, 16400, 21952, 32768, 32784])
+def test_many_long_rows(ops, n):
+    """Enough rows for the threads per row to follow the row's length."""
+    g = _gen(n)
+    x, w = _rand(g, 601, n, std=3.0), _rand(g, n, std=0.2) + 1
+    x[600, n - 1] = 1000.0
+    q, s = ops.quant_fp8(x)
+    ref.check_quant(q, s, x.double(), 2 * ref.F32)
+    no = torch.empty_like(x)
+    q, s, ro = ops.add_rms_norm_fp8(x, w, residual=x, norm_out=no)
+    _check_norm(x, x, w, 1e-6, q, s, ro, no)
+
+
 def test_quant_ties_go_to_even(ops):
     """Half-way values: 448 fixes the scale at 1, so the sums 2^e (8 + m + 1/2) / 8 are exact ties."""
     vals = [2.0 ** e * (8 + m + 0.5) / 8 for e in range(-6, 8) for m in range(8)]
@@ -192,6 +205,23 @@ def test_linear(ops, kind, M, n, K):
                                         ("store", 3, 70000, 256)])
 def test_linear_32b_shapes(ops, kind, M, n, K):
     _check_linear(ops, kind, M, n, K)
+
+
+@pytest.mark.parametrize("kind", ["store", "residual", "swiglu"])
+@pytest.mark.parametrize("M,n,K", [(20, 51201, 64), (33, 40004, 48), (100, 25602, 128), (128, 38400, 144),
+                                   (129, 20001, 80), (300, 12801, 48), (513, 9732, 528), (2049, 5120, 272)])
+def test_linear_many_whole_units(ops, kind, M, n, K):
+    """More weight tiles than CTAs: whole units, odd, even and 8-byte aligned rows, rows past a multiple of 32."""
+    _check_linear(ops, kind, M, n, K)
+
+
+def test_linear_residual_in_place_many_units(ops):
+    g = _gen(12)
+    xq, xs = _quantised(g, 300, 96)
+    wq, ws = _quantised(g, 12801, 96, std=0.05)
+    res = _rand(g, 300, 12801)
+    want = ops.linear_residual_fp8(xq, xs, wq, ws, res)
+    assert torch.equal(ops.linear_residual_fp8(xq, xs, wq, ws, res, out=res), want)
 
 
 def test_linear_strides_and_neighbours(ops):

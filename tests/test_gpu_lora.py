@@ -59,6 +59,17 @@ def test_lora(ops, M, K, slices, R, n_ad, order):
     _check(ops, _case(M, K, slices, R, n_ad, ad))
 
 
+@pytest.mark.parametrize("M,K,slices,R,n_ad", [
+    (1, 8, [8], 128, 1), (2, 264, [96, 32, 32], 40, 3), (16, 520, [72], 64, 16), (17, 520, [72], 64, 17),
+    (31, 5120, [1024, 128, 128], 32, 4), (64, 136, [1000], 64, 64), (65, 1288, [1288], 72, 9),
+    (128, 5120, [5120], 16, 16), (200, 16000, [128], 48, 6), (256, 72, [64, 32], 24, 1), (511, 520, [256], 48, 3),
+    (513, 264, [264], 8, 3)])
+@pytest.mark.parametrize("step", [1, 26, 1000])
+def test_lora_between_the_two_forms(ops, M, K, slices, R, n_ad, step):
+    """Sizes on either side of the choice between one launch and two; rows that alternate, in runs, of one adapter."""
+    _check(ops, _case(M, K, slices, R, n_ad, [(m // step) % n_ad if (m // step) % 5 != 4 else -1 for m in range(M)]))
+
+
 @pytest.mark.parametrize("M", [40, 1400])
 def test_lora_in_place_leaves_other_rows_alone(ops, M):
     st = _case(M, 320, [288, 64], 16, 3, [(m % 4) - 1 for m in range(M)])
