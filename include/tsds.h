@@ -266,7 +266,8 @@ int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const v
  * the columns of each, s(j) is column j's; NULL with one slice.  scale
  * (fp32) and ranks (int32, what an adapter uses of R; the rest of its A and
  * B is not part of the sum, whatever it holds) may be NULL: 1 and R.
- * out may be y (ldo == ldy; rows without an adapter are then not touched).
+ * out may be y (ldo == ldy; rows without an adapter are then not touched),
+ * not x.  Beyond a few rows n_adapters * N < 2^31.
  * Any order of adapters; rows of one request next to one another are
  * fastest.  K % 8 == 0, N % 8 == 0, R % 8 == 0, R <= 128, n_slices <= 4;
  * strides multiples of 8, buffers 16-byte aligned.  An adapter[m] >= n_adapters is not

@@ -89,6 +89,15 @@ def test_lora_codes(lib):
         assert call(**bad) == ALIGN, bad
 
 
+def test_lora_output_over_its_input_and_row_counts(lib):
+    def call(M=2, n_ad=2, x=A, out=A + 65536, N=64):
+        return lib.tsds_lora_add(P(A), N, P(x), 64, P(A), P(A), P(A), None, None, P(out), N, M, 64, N, n_ad, 16, 1, None,
+                                 P(A), 1 << 30, P(A), None)
+    assert call(out=A) == INVALID             # out = y is x as well
+    assert call(x=A + 65536) == INVALID
+    assert call(M=2000, n_ad=1 << 26) == UNSUPPORTED and call(M=2000, n_ad=1 << 20, N=2048) == UNSUPPORTED
+
+
 # -- the Python layer -------------------------------------------------------------
 
 def _cases(t):

@@ -421,7 +421,8 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   TSDS_RETURN_IF(!tsds_aligned16(y) || !tsds_aligned16(x) || !tsds_aligned16(lora_a) || !tsds_aligned16(lora_b) ||
                      !tsds_aligned16(out) || (ldx % 8) || (ldy % 8) || (ldo % 8),
                  TSDS_E_ALIGN);
-  TSDS_RETURN_IF(out == y && ldo != ldy, TSDS_E_INVALID);
+  // x is read while out is written
+  TSDS_RETURN_IF((out == y && ldo != ldy) || out == x, TSDS_E_INVALID);
   p.x = (const bf16*)x;
   p.y = (const bf16*)y;
   p.a = (const bf16*)lora_a;
@@ -443,6 +444,8 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   // 8-byte reads of four rows cover all banks
   p.ld_t = (n_slices * ((R + 15) / 16 * 16) + 63) / 64 * 64 + 16;
   if (!few_rows(M, K, R, n_slices, n_adapters)) {
+    // rows of A and B are tensor-map coordinates there
+    TSDS_RETURN_IF((int64_t)n_adapters * (N > n_slices * R ? N : n_slices * R) > 0x7fffffff, TSDS_E_UNSUPPORTED);
     TSDS_RETURN_IF(!workspace || workspace_bytes < tsds_lora_tc_workspace_bytes(M, R, n_slices), TSDS_E_WORKSPACE);
     TSDS_RETURN_IF(!tsds_aligned16(workspace), TSDS_E_ALIGN);
     return tsds_lora_tc(p, workspace, stream);
