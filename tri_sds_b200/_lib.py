@@ -159,7 +159,7 @@ def exported_symbols() -> list[str]:
 
 def call(name: str, *args) -> None:
     """Call an int-returning entry point; raise on a non-zero status."""
-    lib = load()
+    lib = _lib or load()
     st = getattr(lib, name)(*args)
     if st != 0:
         msg = lib.tsds_status_string(st).decode()

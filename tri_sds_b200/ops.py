@@ -443,6 +443,30 @@ def _vec(t, n: int, what: str) -> None:
         raise ValueError(f"{what} must be contiguous [{n}]")
 
 
+def _fp8_outputs(x, rows, n, out, scale):
+    """q and scale, made or (what the caller gave) checked, and q's row stride."""
+    ldq = n
+    if out is None:
+        out = torch.empty(rows, n, dtype=FP8, device=x.device)
+    else:
+        _cuda(FP8, out)
+        ldq = _ld(out, rows, n, "out")
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    else:
+        _cuda(torch.float32, scale)
+        _vec(scale, rows, "scale")
+    return out, scale, ldq
+
+
+def _bf16_output(x, rows, n, out):
+    """A bf16 [rows, n] output, made or checked, and its row stride."""
+    if out is None:
+        return torch.empty(rows, n, dtype=torch.bfloat16, device=x.device), n
+    _bf16_cuda(out)
+    return out, _ld(out, rows, n, "out")
+
+
 def quant_fp8(x: torch.Tensor, out: torch.Tensor | None = None, scale: torch.Tensor | None = None):
     """Rows of x [rows, n] bf16 to e4m3: (q [rows, n] float8_e4m3fn, scale
     [rows] fp32) with scale = max|x| / 448 of the row, q = e4m3(x / scale).
@@ -450,15 +474,9 @@ def quant_fp8(x: torch.Tensor, out: torch.Tensor | None = None, scale: torch.Ten
     _bf16_cuda(x)
     _need(x.dim() == 2, "x must be [rows, n]")
     rows, n = x.shape
-    if out is None:
-        out = torch.empty(rows, n, dtype=FP8, device=x.device)
-    if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _cuda(FP8, out)
-    _cuda(torch.float32, scale)
-    _vec(scale, rows, "scale")
-    _on(_one_device(x, out, scale), "tsds_quant_fp8", _p(x), _p(out), _p(scale), rows, n, _ld(x, rows, n, "x"),
-        _ld(out, rows, n, "out"))
+    dev = _one_device(x, out, scale)
+    out, scale, ldq = _fp8_outputs(x, rows, n, out, scale)
+    _on(dev, "tsds_quant_fp8", _p(x), _p(out), _p(scale), rows, n, _ld(x, rows, n, "x"), ldq)
     return out, scale
 
 
@@ -473,32 +491,27 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     _bf16_cuda(x, weight, residual, res_out, norm_out)
     _need(x.dim() == 2, "x must be [rows, n]")
     rows, n = x.shape
-    dev = x.device
-    if out is None:
-        out = torch.empty(rows, n, dtype=FP8, device=dev)
-    if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    _cuda(FP8, out)
-    _cuda(torch.float32, scale)
+    dev = _one_device(x, weight, residual, out, scale, res_out, norm_out)
     _vec(weight, n, "weight")
-    _vec(scale, rows, "scale")
     ld_res = ld_out = ld_norm = n
     if residual is None:
         _need(res_out is None, "res_out without a residual")
     else:
+        ld_res = _ld(residual, rows, n, "residual")
         if res_out is None:
-            res_out = torch.empty(rows, n, dtype=torch.bfloat16, device=dev)
-        ld_res, ld_out = _ld(residual, rows, n, "residual"), _ld(res_out, rows, n, "res_out")
+            res_out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
+        else:
+            ld_out = _ld(res_out, rows, n, "res_out")
+    out, scale, ldq = _fp8_outputs(x, rows, n, out, scale)
     if norm_out is not None:
         ld_norm = _ld(norm_out, rows, n, "norm_out")
-    _on(_one_device(x, weight, residual, out, scale, res_out, norm_out), "tsds_add_rms_norm_fp8", _p(x), _p(residual),
-        _p(weight), _p(res_out), _p(out), _p(scale), _p(norm_out), rows, n, _ld(x, rows, n, "x"), ld_res, ld_out,
-        _ld(out, rows, n, "out"), ld_norm, float(eps))
+    _on(dev, "tsds_add_rms_norm_fp8", _p(x), _p(residual), _p(weight), _p(res_out), _p(out), _p(scale), _p(norm_out),
+        rows, n, _ld(x, rows, n, "x"), ld_res, ld_out, ldq, ld_norm, float(eps))
     return out, scale, res_out
 
 
 def _fp8_operands(x, x_scale, w, w_scale, n_out, out):
-    """Checks of the 8-bit projections; returns (M, K, out)."""
+    """Checks of the 8-bit projections; returns (M, K, out, out's row stride)."""
     _cuda(FP8, x, w)
     _cuda(torch.float32, x_scale, w_scale)
     _need(x.dim() == 2, "x must be [M, K]")
@@ -507,11 +520,7 @@ def _fp8_operands(x, x_scale, w, w_scale, n_out, out):
         raise ValueError("w must be contiguous [out, K]")
     _vec(x_scale, M, "x_scale")
     _vec(w_scale, w.shape[0], "w_scale (a scale per row of w)")
-    if out is None:
-        out = torch.empty(M, n_out, dtype=torch.bfloat16, device=x.device)
-    else:
-        _bf16_cuda(out)
-    return M, K, out
+    return M, K, *_bf16_output(x, M, n_out, out)
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -520,9 +529,10 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     (a scale per row) and w [n_out, K] (a scale per output channel)."""
     _need(w.dim() == 2, "w must be [out, K]")
     n_out = w.shape[0]
-    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
-    _on(_one_device(x, x_scale, w, w_scale, out), "tsds_linear_fp8", _p(x), _ld(x, M, K, "x"), _p(x_scale), _p(w),
-        _p(w_scale), _p(out), _ld(out, M, n_out, "out"), M, n_out, K, _p(_scratch.status_word(x.device)))
+    dev = _one_device(x, x_scale, w, w_scale, out)
+    M, K, out, ldo = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
+    _on(dev, "tsds_linear_fp8", _p(x), _ld(x, M, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(out), ldo, M, n_out, K,
+        _p(_scratch.status_word(x.device)))
     return out
 
 
@@ -532,10 +542,10 @@ def linear_residual_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor,
     _need(w.dim() == 2, "w must be [out, K]")
     n_out = w.shape[0]
     _bf16_cuda(res)
-    M, K, out = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
-    _on(_one_device(x, x_scale, w, w_scale, out, res), "tsds_linear_residual_fp8", _p(x), _ld(x, M, K, "x"),
-        _p(x_scale), _p(w), _p(w_scale), _p(res), _ld(res, M, n_out, "res"), _p(out), _ld(out, M, n_out, "out"), M,
-        n_out, K, _p(_scratch.status_word(x.device)))
+    dev = _one_device(x, x_scale, w, w_scale, out, res)
+    M, K, out, ldo = _fp8_operands(x, x_scale, w, w_scale, n_out, out)
+    _on(dev, "tsds_linear_residual_fp8", _p(x), _ld(x, M, K, "x"), _p(x_scale), _p(w), _p(w_scale), _p(res),
+        _ld(res, M, n_out, "res"), _p(out), ldo, M, n_out, K, _p(_scratch.status_word(x.device)))
     return out
 
 
@@ -545,10 +555,10 @@ def linear_swiglu_fp8(x: torch.Tensor, x_scale: torch.Tensor, w_gate_up: torch.T
     ([2I, K] e4m3, 2I scales) -> bf16 [M, I], rounded once."""
     _need(w_gate_up.dim() == 2 and w_gate_up.shape[0] % 2 == 0, "w_gate_up must be [2I, K]")
     I = w_gate_up.shape[0] // 2
-    M, K, out = _fp8_operands(x, x_scale, w_gate_up, w_scale, I, out)
-    _on(_one_device(x, x_scale, w_gate_up, w_scale, out), "tsds_linear_swiglu_fp8", _p(x), _ld(x, M, K, "x"),
-        _p(x_scale), _p(w_gate_up), _p(w_scale), _p(out), _ld(out, M, I, "out"), M, I, K,
-        _p(_scratch.status_word(x.device)))
+    dev = _one_device(x, x_scale, w_gate_up, w_scale, out)
+    M, K, out, ldo = _fp8_operands(x, x_scale, w_gate_up, w_scale, I, out)
+    _on(dev, "tsds_linear_swiglu_fp8", _p(x), _ld(x, M, K, "x"), _p(x_scale), _p(w_gate_up), _p(w_scale), _p(out), ldo,
+        M, I, K, _p(_scratch.status_word(x.device)))
     return out
 
 
@@ -563,7 +573,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     rows of lora_a; ``ranks`` (int32): what each adapter uses of R; ``scale``
     fp32, default 1.  out may be y (in place).  An index past the last adapter
     leaves the row as it is and is reported by check_status()."""
-    _bf16_cuda(y, x, lora_a, lora_b, out)
+    _bf16_cuda(y, x, lora_a, lora_b)
     _cuda(torch.int32, adapter, ranks)
     _cuda(torch.float32, scale)
     _need(y.dim() == 2 and x.dim() == 2 and lora_a.dim() == 3 and lora_b.dim() == 3, "bad dimensions")
@@ -577,13 +587,13 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     for t in (scale, ranks):
         if t is not None:
             _vec(t, n_ad, "scale and ranks (a value per adapter)")
-    if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=y.device)
+    dev = _one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out)
+    out, ldo = _bf16_output(y, M, N, out)
     widths = None if slices is None else (ctypes.c_int32 * S)(*slices)
     nb = _lib.query("tsds_lora_workspace_bytes", M, R, S)
     # of this call alone: calls on several streams and captured graphs share nothing
     ws = torch.empty(nb, dtype=torch.uint8, device=y.device) if nb else None
-    _on(_one_device(y, x, lora_a, lora_b, adapter, scale, ranks, out), "tsds_lora_add", _p(y), _ld(y, M, N, "y"), _p(x),
-        _ld(x, M, K, "x"), _p(lora_a), _p(lora_b), _p(adapter), _p(scale), _p(ranks), _p(out), _ld(out, M, N, "out"),
-        M, K, N, n_ad, R, S, widths, _p(ws), nb, _p(_scratch.status_word(y.device)))
+    _on(dev, "tsds_lora_add", _p(y), _ld(y, M, N, "y"), _p(x), _ld(x, M, K, "x"), _p(lora_a), _p(lora_b), _p(adapter),
+        _p(scale), _p(ranks), _p(out), ldo, M, K, N, n_ad, R, S, widths, _p(ws), nb,
+        _p(_scratch.status_word(y.device)))
     return out
