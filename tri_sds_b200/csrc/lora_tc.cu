@@ -27,8 +27,6 @@
 #include "lora.cuh"
 #include "tc_core.cuh"
 
-#include <type_traits>
-
 using namespace tsds;
 using namespace tsds::tc;
 using namespace tsds::lora;
@@ -70,6 +68,19 @@ __device__ __forceinline__ void tmem_take(uint32_t* to, int columns) {
 }
 __device__ __forceinline__ void tmem_give(uint32_t tmem, int columns) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+}
+
+// A tile of shared memory to global memory, by one thread; stores are waited for in groups.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* smem_src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the last N groups have read their shared memory
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void give_up(int32_t* status, int* abort, int lane) {
@@ -255,24 +266,34 @@ __global__ void __launch_bounds__(THREADS)
   }
 }
 
-constexpr int XN = 64;                      // token rows of an expand unit
-constexpr int X_THREADS = 320;              // TMA warp, MMA warp, two groups of four epilogue warps
-constexpr int B_TILE = TILE_J * 128;        // 128 channels x 64 ranks
-constexpr int T_TILE = XN * 128;            // 64 token rows x 64 ranks
-constexpr int X_LD = 36;                    // padded row of 32 staged channels: 16-byte reads of two rows in all banks
-constexpr int X_STAGING = 8 * 16 * X_LD * (int)sizeof(float);
+constexpr int XM = 128;                     // token rows of an expand block: the MMA's M
+constexpr int X_THREADS = 384;              // B/t warp, MMA warp, y/out warp, an idle one, eight epilogue warps
+constexpr int BOX = XM * 128;               // 128 rows of 128 bytes: of t (64 ranks), B or y (64 channels)
+constexpr int X_SMEM = 208 * 1024 + 1024;   // 1 KB to align
+constexpr int X_BUFS = 2;                   // accumulators
+constexpr int X_RING = 8;                   // most stages of B
 
 struct ExpandArgs {
   LoraArgs l;
-  int ld_t, Rp, blocks, tiles, step, kb;    // step: CTAs that share a block's items; kb: blocks of 64 ranks
+  int ld_t, Rp, tiles, step, kb, tn;        // step: CTAs that share a block's tiles; kb: blocks of 64 ranks; tn: channels per tile
+  int b_stages, y_stages;
   int first_tile[MAX_SLICES + 1];           // channel tiles where the slices begin
   uint64_t wait_ns;
 };
 
+// out, a map per slice: a tile that reaches past its slice's end is cut there
+struct OutMaps {
+  CUtensorMap of[MAX_SLICES];
+};
+
 struct ExpandShared {
-  Tile tile;
-  Adapter group[XN];   // what this CTA adds or copies, in turn
-  uint64_t t_full, full[2], empty[2], tfull[2], tempty[2], drain;
+  alignas(16) int32_t id[XM];   // adapter of each row; -1: none; -2: past the last row
+  int32_t group[XM];            // its place among the block's adapters; -1: nothing to add
+  int32_t gid[XM], grank[XM];   // the block's adapters: index, rank
+  int32_t rank[NEAR];           // rank of the first adapters
+  uint32_t leads[4];            // bits of the rows that are the first of their adapter
+  int plain;                    // a row without an adapter
+  uint64_t full[X_RING], empty[X_RING], t_full, t_empty, tfull[X_BUFS], tempty[X_BUFS], yfull[4], ydone[4], drain;
   uint32_t tmem;
   int abort;
 };
@@ -287,253 +308,293 @@ __device__ __forceinline__ Channels channels_of(const ExpandArgs& p, int tile) {
 #pragma unroll
   for (int i = 1; i < MAX_SLICES; ++i)
     if (i < p.l.S && tile >= p.first_tile[i]) c.sl = i;
-  c.lo = p.l.first_col[c.sl] + (tile - p.first_tile[c.sl]) * TILE_J;
+  c.lo = p.l.first_col[c.sl] + (tile - p.first_tile[c.sl]) * p.tn;
   c.end = p.l.first_col[c.sl + 1];
   return c;
 }
 
-// An item of expand's work: one adapter of the block and a channel tile.  The CTA
-// of index c takes items c, c + step, ... of all of them, adapter by adapter.
-struct Item {
-  int g, tile;
-};
-__device__ __forceinline__ Item next_item(const ExpandArgs& p, Item it) {
-  for (it.tile += p.step; it.tile >= p.tiles; it.tile -= p.tiles) ++it.g;
-  return it;
+// The block's rows by adapter, by the first 128 threads (the next 64 read ranks
+// meanwhile); returns how many adapters have something to add.
+__device__ __forceinline__ int group_block(const ExpandArgs& p, ExpandShared& sh, int row0) {
+  const LoraArgs& l = p.l;
+  const int tid = threadIdx.x, lane = tid & 31;
+  int id = -2, m = row0 + tid;
+  if (tid < XM) {
+    if (m < l.M) {
+      id = l.adapter[m];
+      if (id < 0 || id >= l.n_adapters) id = -1;   // (shrink has reported an index past the last)
+    }
+    sh.id[tid] = id;
+  } else if (tid < XM + NEAR) {
+    const int a = tid - XM;
+    sh.rank[a] = l.ranks && a < l.n_adapters ? l.ranks[a] : l.R;
+  }
+  if (tid == 0) sh.plain = 0;
+  __syncthreads();
+  int ra = 0, first = tid;
+  if (tid < XM) {
+    if (id >= 0) ra = id < NEAR ? sh.rank[id] : (l.ranks ? l.ranks[id] : l.R);
+    ra = ra < 0 ? 0 : (ra > l.R ? l.R : ra);
+#pragma unroll 4
+    for (int j = XM - 4; j >= 0; j -= 4) {   // without a branch; the smallest row comes last
+      const int4 v = *reinterpret_cast<const int4*>(sh.id + j);
+      first = v.w == id ? j + 3 : first;
+      first = v.z == id ? j + 2 : first;
+      first = v.y == id ? j + 1 : first;
+      first = v.x == id ? j : first;
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, ra > 0 && first == tid);
+    if (lane == 0) sh.leads[tid >> 5] = bits;
+    if (id != -2 && ra == 0) sh.plain = 1;
+  }
+  __syncthreads();
+  auto before = [&](int row) {
+    int n = __popc(sh.leads[row >> 5] & ((1u << (row & 31)) - 1));
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+      if (w < row >> 5) n += __popc(sh.leads[w]);
+    return n;
+  };
+  if (tid < XM) {
+    const int g = before(first);
+    sh.group[tid] = ra > 0 ? g : -1;
+    if (ra > 0 && first == tid) {
+      sh.gid[g] = id;
+      sh.grank[g] = ra;
+    }
+  }
+  __syncthreads();
+  return __popc(sh.leads[0]) + __popc(sh.leads[1]) + __popc(sh.leads[2]) + __popc(sh.leads[3]);
 }
 
-__global__ void __launch_bounds__(X_THREADS, 2)
-    expand_kernel(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap tmap, ExpandArgs p) {
+template <int PER_SM>   // CTAs per SM
+__global__ void __launch_bounds__(X_THREADS, PER_SM)
+    expand_kernel(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap tmap,
+                  const __grid_constant__ CUtensorMap ymap, const __grid_constant__ OutMaps omap, ExpandArgs p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ ExpandShared sh;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (warp == 1) tmem_take(&sh.tmem, 2 * XN);
-  const int block = blockIdx.x / p.step, row0 = block * XN;
-  const int index = blockIdx.x - block * p.step;
-  const Item first = {index / p.tiles, index % p.tiles};
-  if (warp == 0 && elect_one()) {
-    prefetch_tmap(&bmap);
-    prefetch_tmap(&tmap);
-    mbar_init(&sh.t_full, 1);
-    for (int i = 0; i < 2; ++i) {
+  if (warp == 1) tmem_take(&sh.tmem, X_BUFS * p.tn);
+  const int block = blockIdx.x / p.step, row0 = block * XM, tile0 = blockIdx.x - block * p.step;
+  const int items = (p.tiles - tile0 + p.step - 1) / p.step, boxes = p.tn / 64;
+  uint8_t *t_smem = smem, *b_smem = t_smem + p.kb * 2 * BOX, *y_smem = b_smem + p.b_stages * p.kb * p.tn * 128;
+  auto load_y = [&](int i) {   // by one thread
+    const int s = i % p.y_stages, lo = channels_of(p, tile0 + i * p.step).lo;
+    mbar_arrive_expect_tx(&sh.yfull[s], boxes * BOX);
+    for (int h = 0; h < boxes; ++h) tma_load_2d(y_smem + (s * boxes + h) * BOX, &ymap, &sh.yfull[s], lo + h * 64, row0);
+  };
+  if (warp == 2 && lane == 0) {
+    for (int i = 0; i < X_RING; ++i) {
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);
-      mbar_init(&sh.tfull[i], 1);
-      mbar_init(&sh.tempty[i], 8);   // one arrival per epilogue warp
     }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.yfull[i], 1);
+      mbar_init(&sh.ydone[i], 8);    // one arrival per epilogue warp
+    }
+    for (int i = 0; i < X_BUFS; ++i) {
+      mbar_init(&sh.tfull[i], 1);
+      mbar_init(&sh.tempty[i], 8);
+    }
+    mbar_init(&sh.t_full, 1);
+    mbar_init(&sh.t_empty, 1);
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     fence_barrier_init();
+    fence_proxy_async();
+    for (int i = 0; i < items && i < p.y_stages; ++i) load_y(i);   // y is complete before shrink starts
   }
   tc_fence_before();
   pdl_trigger();
-  group_rows(p.l, sh.tile, row0, XN, false, p.l.out != p.l.y);
+  const int groups = group_block(p, sh, row0);
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const int groups = __popcll(sh.tile.leads);
-  if (groups <= first.g) {   // nothing for this CTA
-    if (warp == 1) tmem_give(tmem, 2 * XN);
-    pdl_wait();
-    return;
-  }
-  if (threadIdx.x < XN && (sh.tile.leads >> threadIdx.x & 1)) {
-    const int i = __popcll(sh.tile.leads & ((1ull << threadIdx.x) - 1)), id = sh.tile.id[threadIdx.x];
-    sh.group[i] = id >= 0 ? adapter_of(p.l, sh.tile, id) : Adapter{id, 0, 0.f};
-  }
-  __syncthreads();
-  const int b_bytes = p.kb * B_TILE;
-  uint8_t *b_smem = smem, *t_smem = smem + 2 * b_bytes;   // t: [slice][kb][hi, lo]
-  float* stg = reinterpret_cast<float*>(t_smem + p.l.S * p.kb * 2 * T_TILE);
-  int buf = 0, issued = 0;     // ring position = accumulator: one B tile per output tile
-  uint32_t phase = 0;
+  // rows without an adapter stay as they are where out is y: then rows are
+  // stored one by one
+  const bool in_place = p.l.out == p.l.y, by_row = in_place && sh.plain;
+  const bool any = groups > 0 || !in_place;
+  int issued = 0, slices = 0;   // blocks of the B ring (warps 0 and 1), loads of t (warp 0)
+  int y_issued = items < p.y_stages ? items : p.y_stages;
   bool ok = true;
 
-  // every warp goes through the same items, group by group and tile by tile,
-  // without a barrier between groups
   if (warp == 0) {
-    for (Item it = first; it.g < groups; it = next_item(p, it)) {
-      const Adapter ad = sh.group[it.g];
-      if (ad.ra == 0) continue;
-      ok = warp_wait(&sh.empty[buf], phase ^ 1, p.wait_ns);
-      if (!ok) break;
-      if (elect_one()) {
-        const int kb = (ad.ra + BKE - 1) / BKE;
-        mbar_arrive_expect_tx(&sh.full[buf], kb * B_TILE);
-        for (int i = 0; i < kb; ++i)
-          tma_load_2d(b_smem + buf * b_bytes + i * B_TILE, &bmap, &sh.full[buf], i * BKE,
-                      ad.id * p.l.N + channels_of(p, it.tile).lo);
-      }
-      __syncwarp();
-      if (issued == 0) {   // every slice's t of these rows, once; the first read that waits for shrink
-        pdl_wait();
+    int s = 0, sl = -1;
+    uint32_t phase = 1;
+    for (int i = 0; ok && i < items && groups > 0; ++i) {
+      const Channels c = channels_of(p, tile0 + i * p.step);
+      for (int g = 0; g < groups; ++g) {
+        ok = warp_wait(&sh.empty[s], phase, p.wait_ns);
+        if (!ok) break;
+        const int id = sh.gid[g], kb = (sh.grank[g] + BKE - 1) / BKE;
         if (elect_one()) {
-          mbar_arrive_expect_tx(&sh.t_full, p.l.S * p.kb * 2 * T_TILE);
-          for (int i = 0; i < p.l.S * p.kb; ++i) {
-            uint8_t* t = t_smem + i * 2 * T_TILE;
-            tma_load_2d(t, &tmap, &sh.t_full, i * BKE, row0);
-            tma_load_2d(t + T_TILE, &tmap, &sh.t_full, p.ld_t + i * BKE, row0);
+          mbar_arrive_expect_tx(&sh.full[s], kb * p.tn * 128);
+          for (int k = 0; k < kb; ++k)
+            tma_load_2d(b_smem + (s * p.kb + k) * p.tn * 128, &bmap, &sh.full[s], k * BKE, id * p.l.N + c.lo);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == p.b_stages) {
+          s = 0;
+          phase ^= 1;
+        }
+        if (sl != c.sl) {   // the slice's t; the first read that waits for shrink
+          if (slices == 0)
+            pdl_wait();
+          else
+            ok = warp_wait(&sh.t_empty, (slices - 1) & 1, p.wait_ns);
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&sh.t_full, p.kb * 2 * BOX);
+            for (int k = 0; k < p.kb * 2; ++k)   // hi, lo of each 64 ranks
+              tma_load_2d(t_smem + k * BOX, &tmap, &sh.t_full, (k & 1) * p.ld_t + c.sl * p.Rp + (k >> 1) * BKE, row0);
+          }
+          __syncwarp();
+          sl = c.sl;
+          ++slices;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc =
+        (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.tn >> 3) << 17) | ((uint32_t)(XM >> 4) << 24);
+    const uint64_t t0 = sdesc_sw128(smem_u32(t_smem));
+    int s = 0, sl = -1, buf = 0;
+    uint32_t phase = 0, tphase = 1, slice_phase = 1;
+    for (int i = 0; ok && i < items && groups > 0; ++i) {
+      const Channels c = channels_of(p, tile0 + i * p.step);
+      if (sl != c.sl) {
+        if (sl >= 0 && elect_one()) umma_commit(&sh.t_empty);   // the old slice's products are done
+        __syncwarp();
+        sl = c.sl;
+        slice_phase ^= 1;
+        ok = warp_wait(&sh.t_full, slice_phase, p.wait_ns);
+      }
+      for (int g = 0; ok && g < groups; ++g) {
+        ok = warp_wait(&sh.tempty[buf], tphase, p.wait_ns) && warp_wait(&sh.full[s], phase, p.wait_ns);
+        if (!ok) break;
+        const int ra = sh.grank[g], steps = (ra + 15) / 16;   // of 16 ranks
+        uint8_t* bs = b_smem + s * p.kb * p.tn * 128;
+        if (ra & 15) {
+          // the last step's ranks past the adapter's: B's columns there are not
+          // part of it, whatever they hold
+          const int from = ra & 63, to = ((ra + 15) & ~15) - (ra & ~63);
+          uint8_t* b = bs + (ra / 64) * p.tn * 128;
+          for (int row = lane; row < p.tn; row += 32)
+            for (int k = from; k < to; ++k)
+              *reinterpret_cast<uint16_t*>(b + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 7) * 2) = 0;
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (elect_one()) {
+          tc_fence_after();
+          const uint64_t b0 = sdesc_sw128(smem_u32(bs));
+          for (int k = 0; k < steps; ++k) {
+            const uint64_t b = b0 + (uint32_t)((k >> 2) * p.tn * 128 >> 4) + (k & 3) * 2;
+            const uint64_t t = t0 + (uint32_t)((k >> 2) * 2 * BOX >> 4) + (k & 3) * 2;
+            umma_bf16(tmem + buf * p.tn, t + (BOX >> 4), b, idesc, k != 0);   // lo
+            umma_bf16(tmem + buf * p.tn, t, b, idesc, 1);                     // hi
+          }
+          umma_commit(&sh.empty[s]);
+          umma_commit(&sh.tfull[buf]);
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == p.b_stages) {
+          s = 0;
+          phase ^= 1;
+        }
+        if (++buf == X_BUFS) {
+          buf = 0;
+          tphase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 2) {
+    if (any) {
+      pdl_wait();   // what is stored may be what an earlier kernel still reads
+      for (int i = 0; i < items; ++i) {
+        ok = warp_wait(&sh.ydone[i % p.y_stages], (i / p.y_stages) & 1, p.wait_ns);
+        if (!ok) break;
+        if (lane == 0) {
+          const Channels c = channels_of(p, tile0 + i * p.step);
+          for (int h = 0; h < boxes && !by_row; ++h) {
+            const int x = c.lo + h * 64;
+            if (x < c.end)
+              tma_store_2d(&omap.of[c.sl], x - p.l.first_col[c.sl], row0,
+                           y_smem + (i % p.y_stages * boxes + h) * BOX);
+          }
+          bulk_commit();
+          if (i > 0 && i - 1 + p.y_stages < items) {
+            bulk_wait_read<1>();   // the item before has left its stage
+            load_y(i - 1 + p.y_stages);
           }
         }
         __syncwarp();
+        if (i > 0 && i - 1 + p.y_stages < items) ++y_issued;
       }
-      ++issued;
-      phase ^= buf;
-      buf ^= 1;
     }
-  } else if (warp == 1) {
-    for (Item it = first; it.g < groups; it = next_item(p, it)) {
-      const Adapter ad = sh.group[it.g];
-      const int steps = (ad.ra + 15) / 16;   // of 16 ranks
-      if (steps == 0) continue;
-      ok = warp_wait(&sh.tempty[buf], phase ^ 1, p.wait_ns) && warp_wait(&sh.full[buf], phase, p.wait_ns) &&
-           warp_wait(&sh.t_full, 0, p.wait_ns);
-      if (!ok) break;
-      uint8_t* bs = b_smem + buf * b_bytes;
-      if (ad.ra & 15) {
-        // the last step's ranks past the adapter's: B's columns there are not
-        // part of it, whatever they hold
-        const int from = ad.ra & 63, to = ((ad.ra + 15) & ~15) - (ad.ra & ~63);
-        uint8_t* b = bs + (ad.ra / 64) * B_TILE;
-        for (int row = lane; row < TILE_J; row += 32)
-          for (int c = from; c < to; ++c)
-            *reinterpret_cast<uint16_t*>(b + row * 128 + (((c >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0;
-        fence_proxy_async();
-      }
-      __syncwarp();
-      if (elect_one()) {
+  } else if (warp >= 4 && any) {
+    // A lane is a token row: it adds its adapter's products to its row of the
+    // y tile in shared memory, half of the tile's channels, 32 at a time.
+    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane, cols = p.tn / 2;
+    const int mine = sh.group[row];
+    bf16* out_row = p.l.out + (int64_t)(row0 + row) * p.l.ldo;
+    int buf = 0;
+    uint32_t tphase = 0;
+    for (int i = 0; ok && i < items; ++i) {
+      const int st = i % p.y_stages;
+      ok = warp_wait(&sh.yfull[st], (i / p.y_stages) & 1, p.wait_ns);
+      const Channels ch = channels_of(p, tile0 + i * p.step);
+      for (int g = 0; ok && g < groups; ++g) {
+        ok = warp_wait(&sh.tfull[buf], tphase, p.wait_ns);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t idesc =
-            (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(XN >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
-        const uint64_t b0 = sdesc_sw128(smem_u32(bs));
-        const uint64_t t0 = sdesc_sw128(smem_u32(t_smem + channels_of(p, it.tile).sl * p.kb * 2 * T_TILE));
-        for (int i = 0; i < steps; ++i) {
-          const uint64_t b = b0 + (uint32_t)((i >> 2) * B_TILE >> 4) + (i & 3) * 2;
-          const uint64_t t = t0 + (uint32_t)((i >> 2) * 2 * T_TILE >> 4) + (i & 3) * 2;
-          umma_bf16(tmem + buf * XN, b, t + (T_TILE >> 4), idesc, i != 0);   // lo
-          umma_bf16(tmem + buf * XN, b, t, idesc, 1);                        // hi
-        }
-        umma_commit(&sh.empty[buf]);
-        umma_commit(&sh.tfull[buf]);
-      }
-      __syncwarp();
-      ++issued;
-      phase ^= buf;
-      buf ^= 1;
-    }
-  } else {
-    // A warp takes 32 channels (its lanes of TMEM) of 32 token rows, a thread
-    // eight channels of every eighth row, so a warp accesses rows in runs of 64
-    // bytes.  It transposes 16 rows at a time through staging of its own: with
-    // 128 threads on one staging area and a branch per row an item took twice as long.
-    const int half = (warp - 2) >> 2, quarter = warp & 3;
-    const int tr = half * 32 + (lane >> 2), j0 = quarter * 32 + (lane & 3) * 8;
-    float* to = stg + (warp - 2) * 16 * X_LD + lane;
-    const float* from = stg + (warp - 2) * 16 * X_LD + (lane >> 2) * X_LD + (lane & 3) * 8;
-    using Yes = std::true_type;
-    using No = std::false_type;
-    const int row_id = sh.tile.id[half * 32 + lane];
-    struct Part {   // an item's part of this warp
-      int id, lo;
-      bool whole, in;   // all 32 x 32 outputs, any of this thread's channels
-    };
-    auto part_of = [&](Item it) {
-      const Channels c = channels_of(p, it.tile);
-      Part w;
-      w.id = sh.group[it.g].id;
-      w.lo = c.lo;
-      w.in = c.lo + j0 < c.end;
-      w.whole = __all_sync(0xffffffffu, row_id == w.id && w.in);
-      return w;
-    };
-    auto load_y = [&](Item it, uint4 (&y)[4]) {
-      if (it.g >= groups) return;
-      const Part w = part_of(it);
-      const bf16* at = p.l.y + (int64_t)(row0 + tr) * p.l.ldy + w.lo + j0;
-      if (w.whole) {
+        if (__any_sync(0xffffffffu, mine == g)) {
+          for (int c = 0; c < cols; c += 32) {
+            const int col = half * cols + c;   // of the tile
+            uint32_t v[32];
+            tmem_request32(tmem + buf * p.tn + ((uint32_t)(quarter * 32) << 16) + col, v);
+            uint8_t* box = y_smem + (st * boxes + (col >> 6)) * BOX + row * 128;
+            uint4* at[4];
+            uint4 y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
-      } else {
+            for (int k = 0; k < 4; ++k) {
+              at[k] = reinterpret_cast<uint4*>(box + (((((col & 63) >> 3) + k) ^ (row & 7)) << 4));
+              y[k] = *at[k];
+            }
+            tmem_wait32(v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (w.in && sh.tile.id[tr + i * 8] == w.id) y[i] = *reinterpret_cast<const uint4*>(at + i * 8 * p.l.ldy);
-      }
-    };
-    // an item further ahead: its lines into L2, one per thread of every other warp
-    auto prefetch_y = [&](Item it) {
-      if (it.g >= groups || (quarter & 1) || row_id != sh.group[it.g].id) return;
-      const Channels c = channels_of(p, it.tile);
-      if (c.lo + quarter * 32 < c.end)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.l.y + (int64_t)(row0 + half * 32 + lane) * p.l.ldy + c.lo +
-                                                      quarter * 32));
-    };
-    auto finish = [&](Item it, const uint4 (&y)[4]) {
-      const Part w = part_of(it);
-      bf16* out = p.l.out + (int64_t)(row0 + tr) * p.l.ldo + w.lo + j0;
-      if (sh.group[it.g].ra == 0) {
+            for (int k = 0; k < 4; ++k) {
+              const float* d = reinterpret_cast<const float*>(v) + k * 8;
+              y[k] = make_uint4(pack_bf2(bf_lo(y[k].x) + d[0], bf_hi(y[k].x) + d[1]),
+                                pack_bf2(bf_lo(y[k].y) + d[2], bf_hi(y[k].y) + d[3]),
+                                pack_bf2(bf_lo(y[k].z) + d[4], bf_hi(y[k].z) + d[5]),
+                                pack_bf2(bf_lo(y[k].w) + d[6], bf_hi(y[k].w) + d[7]));
+            }
+            if (mine == g) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (w.in && sh.tile.id[tr + i * 8] == w.id) *reinterpret_cast<uint4*>(out + i * 8 * p.l.ldo) = y[i];
-        return;
-      }
-      ok = warp_wait(&sh.tfull[buf], phase, p.wait_ns);
-      if (!ok) return;
-      tc_fence_after();
-      uint32_t v[32];
-      tmem_request32(tmem + buf * XN + ((uint32_t)(quarter * 32) << 16) + half * 32, v);
-      tmem_wait32(v);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.tempty[buf]);   // this warp has read its part of the accumulator
-      auto rest = [&](auto whole) {
-#pragma unroll
-        for (int c = 0; c < 32; c += 16) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) to[i * X_LD] = __uint_as_float(v[c + i]);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int k = c / 8 + i;
-            const float4 a = *reinterpret_cast<const float4*>(from + i * 8 * X_LD);
-            const float4 b = *reinterpret_cast<const float4*>(from + i * 8 * X_LD + 4);
-            const uint4 o = y[k];
-            if (whole || (w.in && sh.tile.id[tr + k * 8] == w.id))
-              *reinterpret_cast<uint4*>(out + k * 8 * p.l.ldo) = make_uint4(
-                  pack_bf2(bf_lo(o.x) + a.x, bf_hi(o.x) + a.y), pack_bf2(bf_lo(o.y) + a.z, bf_hi(o.y) + a.w),
-                  pack_bf2(bf_lo(o.z) + b.x, bf_hi(o.z) + b.y), pack_bf2(bf_lo(o.w) + b.z, bf_hi(o.w) + b.w));
+              for (int k = 0; k < 4; ++k) {
+                if (!by_row)
+                  *at[k] = y[k];
+                else if (ch.lo + col + k * 8 < ch.end)
+                  *reinterpret_cast<uint4*>(out_row + ch.lo + col + k * 8) = y[k];
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
-      };
-      if (w.whole)
-        rest(Yes());
-      else
-        rest(No());
-      phase ^= buf;
-      buf ^= 1;
-    };
-    // the next item's y is requested before this one's is used, in a register
-    // set of its own: loads are awaited by set, so one set would be awaited
-    // with the requests just made (5 us a tile instead of 1.2)
-    uint4 y0[4], y1[4];
-    Item now = first, next = next_item(p, now), ahead = next_item(p, next);
-    load_y(now, y0);
-    prefetch_y(next);
-    prefetch_y(ahead);
-    pdl_wait();   // a copied row may be what an earlier kernel still reads
-    while (now.g < groups) {
-      ahead = next_item(p, ahead);
-      load_y(next, y1);
-      prefetch_y(ahead);
-      finish(now, y0);
-      if (!ok || next.g >= groups) break;
-      now = next_item(p, next);
-      ahead = next_item(p, ahead);
-      load_y(now, y0);
-      prefetch_y(ahead);
-      finish(next, y1);
-      if (!ok) break;
-      next = next_item(p, now);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.tempty[buf]);
+        if (++buf == X_BUFS) {
+          buf = 0;
+          tphase ^= 1;
+        }
+      }
+      fence_proxy_async();   // the store reads what this warp wrote
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(&sh.ydone[st]);
     }
   }
   if (!ok) {
@@ -542,19 +603,24 @@ __global__ void __launch_bounds__(X_THREADS, 2)
   }
   __syncwarp();
   pdl_wait();
+  if (warp == 2 && lane == 0) {
+    bulk_wait_read<0>();
+    if (!any) drain_tma_ring(sh.yfull, p.y_stages, y_issued);   // nothing waited for them
+  }
   tc_fence_before();
   __syncthreads();
   if (sh.abort) {   // uniform: copies and MMAs in flight finish (bounded) before TMEM is freed
     if (warp == 0 && lane == 0) {
-      drain_tma_ring(sh.full, 2, issued);
-      if (issued > 0) mbar_wait(&sh.t_full, 0, 20000000ull);   // requested behind the first tile
+      drain_tma_ring(sh.full, p.b_stages, issued);
+      if (slices > 0) mbar_wait(&sh.t_full, (slices - 1) & 1, 20000000ull);
     }
+    if (warp == 2 && lane == 0) drain_tma_ring(sh.yfull, p.y_stages, y_issued);
     if (warp == 1 && lane == 0 && issued > 0) drain_mma<1>(&sh.drain);
     __syncthreads();
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_give(tmem, 2 * XN);
+    tmem_give(tmem, X_BUFS * p.tn);
   }
 }
 
@@ -564,10 +630,21 @@ int launch_shrink(const CUtensorMap& a_all, const CUtensorMap& a_box, const CUte
   const int st = tsds_smem_limit_once(shrink_kernel, 97 * 1024, limit_set);
   if (st != TSDS_OK) return st;
   // more of the SM's shared memory than of TMEM's columns (at least 57 KB for 64;
-  // expand: 65 KB for 128), so CTAs that fit an SM never wait for columns
+  // expand: 200 KB for 256, 89 KB for 128), so CTAs that fit an SM never wait for columns
   const int smem = p.stages * p.stage_bytes + A_SLACK + 1024;
   tsds_launch_cluster(shrink_kernel, dim3((unsigned)(p.blocks * p.l.slots * CL)), dim3(THREADS), smem, stream, CL,
                       a_all, a_box, xmap, p);
+  return tsds_launch_status();
+}
+
+template <int PER_SM>
+int launch_expand(const CUtensorMap& bmap, const CUtensorMap& tmap, const CUtensorMap& ymap, const OutMaps& omap,
+                  const ExpandArgs& p, int blocks, int smem, cudaStream_t stream) {
+  static tsds_device_flags limit_set;
+  const int st = tsds_smem_limit_once(expand_kernel<PER_SM>, X_SMEM, limit_set);
+  if (st != TSDS_OK) return st;
+  tsds_launch(expand_kernel<PER_SM>, dim3((unsigned)(blocks * p.step)), dim3(X_THREADS), smem, stream, bmap, tmap, ymap,
+              omap, p);
   return tsds_launch_status();
 }
 
@@ -608,39 +685,62 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.l.slots = 2 * sms / CL / p.blocks;
   p.l.slots = p.l.slots < 1 ? 1 : (p.l.slots > p.nt ? p.nt : p.l.slots);
   if (p.l.slots > l.n_adapters) p.l.slots = l.n_adapters;
-  CUtensorMap a_all, a_box, xmap, bmap, tmap;
+  CUtensorMap a_all, a_box, xmap, bmap, tmap, ymap;
   const uint64_t a_rows = (uint64_t)l.n_adapters * SR;
   int st = tsds_make_tmap_2d_bf16(&a_all, l.a, l.K, a_rows, (uint64_t)l.K * 2, BKE, p.arows, 1);
   if (st == TSDS_OK) st = tsds_make_tmap_2d_bf16(&a_box, l.a, l.K, a_rows, (uint64_t)l.K * 2, BKE, p.bx, 1);
   if (st == TSDS_OK) st = tsds_make_tmap_2d_bf16(&xmap, l.x, l.K, l.M, (uint64_t)l.ldx * 2, BKE, p.nt, 1);
+  ExpandArgs q = {};
+  q.l = l;
+  q.ld_t = p.ld_t;
+  q.Rp = p.Rp;
+  q.kb = p.Rp / BKE;
+  q.wait_ns = p.wait_ns;
+  // 128 channels per tile and one CTA per SM with deep rings; but 64 and two
+  // CTAs per SM (where their t leaves room) with few tiles and several adapters in a
+  // block: they follow one another in a tile (64 rows that alternate between 8 adapters
+  // of rank 64 into q/k/v 23.3 us instead of 25.5; of one adapter it is 13.4 instead of 12.7).
+  const int blocks = (l.M + XM - 1) / XM;
+  auto shape = [&](int tn, int places) {
+    q.tn = tn;
+    for (int i = 0; i < l.S; ++i)
+      q.first_tile[i + 1] = q.first_tile[i] + (l.first_col[i + 1] - l.first_col[i] + tn - 1) / tn;
+    q.tiles = q.first_tile[l.S];
+    int step = places / blocks;
+    step = step < 1 ? 1 : (step > q.tiles ? q.tiles : step);
+    const int per = (q.tiles + step - 1) / step;
+    q.step = (q.tiles + per - 1) / per;   // the tiles evenly among the CTAs
+    return per;
+  };
+  int budget = X_SMEM, per = shape(128, sms);
+  bool two = false;
+  if (per <= 2 && l.n_adapters > 2 * blocks) {
+    two = q.kb == 1;
+    per = shape(64, two ? 2 * sms : sms);
+    if (two) budget = 112 * 1024;
+  }
+  const int b_stage = q.kb * q.tn * 128, y_stage = q.tn / 64 * BOX;
+  budget -= 1024 + q.kb * 2 * BOX;
+  q.y_stages = (budget - 2 * b_stage) / y_stage;
+  q.y_stages = q.y_stages > 4 ? 4 : q.y_stages;
+  if (q.y_stages > per) q.y_stages = per < 2 ? 2 : per;
+  q.b_stages = (budget - q.y_stages * y_stage) / b_stage;
+  if (q.b_stages > X_RING) q.b_stages = X_RING;
+  const int smem = 1024 + q.kb * 2 * BOX + q.b_stages * b_stage + q.y_stages * y_stage;
+  OutMaps omap;
   if (st == TSDS_OK)
-    st = tsds_make_tmap_2d_bf16(&bmap, l.b, l.R, (uint64_t)l.n_adapters * l.N, (uint64_t)l.R * 2, BKE, TILE_J, 1);
+    st = tsds_make_tmap_2d_bf16(&bmap, l.b, l.R, (uint64_t)l.n_adapters * l.N, (uint64_t)l.R * 2, BKE, q.tn, 1);
   if (st == TSDS_OK)
-    st = tsds_make_tmap_2d_bf16(&tmap, workspace, 2 * (uint64_t)p.ld_t, l.M, 4 * (uint64_t)p.ld_t, BKE, XN, 1);
+    st = tsds_make_tmap_2d_bf16(&tmap, workspace, 2 * (uint64_t)p.ld_t, l.M, 4 * (uint64_t)p.ld_t, BKE, XM, 1);
+  if (st == TSDS_OK) st = tsds_make_tmap_2d_bf16(&ymap, l.y, l.N, l.M, (uint64_t)l.ldy * 2, 64, XM, 1);
+  for (int i = 0; i < l.S && st == TSDS_OK; ++i)
+    st = tsds_make_tmap_2d_bf16(&omap.of[i], l.out + l.first_col[i], l.first_col[i + 1] - l.first_col[i], l.M,
+                                (uint64_t)l.ldo * 2, 64, XM, 1);
   if (st != TSDS_OK) return st;
 
   st = launch_shrink(a_all, a_box, xmap, p, stream);
   if (st != TSDS_OK) return st;
 
-  ExpandArgs q = {};
-  q.l = l;
-  q.ld_t = p.ld_t;
-  q.Rp = p.Rp;
-  q.blocks = (l.M + XN - 1) / XN;
-  q.kb = p.Rp / BKE;
-  for (int i = 0; i < l.S; ++i)
-    q.first_tile[i + 1] = q.first_tile[i] + (l.first_col[i + 1] - l.first_col[i] + TILE_J - 1) / TILE_J;
-  q.tiles = q.first_tile[l.S];
-  q.wait_ns = p.wait_ns;
-  const int smem = 2 * q.kb * B_TILE + l.S * q.kb * 2 * T_TILE + X_STAGING + 1024;
-  // a block's items over as many CTAs as are resident at once
-  const int places = sms * (smem <= 112 * 1024 ? 2 : 1), most = q.tiles * (l.n_adapters < XN ? l.n_adapters + 1 : XN);
-  q.step = places / q.blocks;
-  q.step = q.step < 1 ? 1 : (q.step > most ? most : q.step);
-  static tsds_device_flags expand_set;
-  st = tsds_smem_limit_once(expand_kernel, 220 * 1024, expand_set);
-  if (st != TSDS_OK) return st;
-  tsds_launch(expand_kernel, dim3((unsigned)(q.blocks * q.step)), dim3(X_THREADS), smem, stream, bmap, tmap,
-              q);
-  return tsds_launch_status();
+  return two ? launch_expand<2>(bmap, tmap, ymap, omap, q, blocks, smem, stream)
+             : launch_expand<1>(bmap, tmap, ymap, omap, q, blocks, smem, stream);
 }
