@@ -70,6 +70,22 @@ def test_lora_between_the_two_forms(ops, M, K, slices, R, n_ad, step):
     _check(ops, _case(M, K, slices, R, n_ad, [(m // step) % n_ad if (m // step) % 5 != 4 else -1 for m in range(M)]))
 
 
+@pytest.mark.parametrize("M,K,slices,R,n_ad", [
+    (3600, 72, [96, 32], 24, 3), (3585, 520, [264], 8, 40), (4100, 264, [32, 64, 96, 32], 40, 130),
+    (2048, 136, [160, 32], 128, 5), (150, 264, [1088, 32, 96], 64, 150), (600, 1032, [328], 96, 600)])
+@pytest.mark.parametrize("step", [1, 70, 5000])
+def test_lora_blocks_of_many_rows(ops, M, K, slices, R, n_ad, step):
+    """Blocks of 128 rows with one adapter or up to 128, in and out of place, with and without rows that have none."""
+    st = _case(M, K, slices, R, n_ad, [(m // step) % n_ad if (m // step) % 7 != 6 else -1 for m in range(M)])
+    want = _check(ops, st)
+    y = st["y"].clone()
+    assert torch.equal(ops.lora_add(**dict(st, y=y), out=y), want)
+    st["adapter"] = st["adapter"].clamp(min=0)
+    want = _check(ops, st)
+    y = st["y"].clone()
+    assert torch.equal(ops.lora_add(**dict(st, y=y), out=y), want)
+
+
 @pytest.mark.parametrize("M", [40, 1400])
 def test_lora_in_place_leaves_other_rows_alone(ops, M):
     st = _case(M, 320, [288, 64], 16, 3, [(m % 4) - 1 for m in range(M)])

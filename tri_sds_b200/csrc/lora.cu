@@ -331,10 +331,10 @@ __global__ void __launch_bounds__(F::THREADS, F::CTAS) lora_kernel(LoraArgs p) {
   pdl_trigger();
   pdl_wait();
   group_rows(p, sh, row0, TR, rank == 0, p.out != p.y);
-  unsigned long long leads = sh.leads;
+  uint32_t leads = sh.leads[0];   // TR rows
   for (int gi = 0; leads; ++gi, leads &= leads - 1) {
     if (gi % p.slots != slot) continue;
-    const int id = sh.id[__ffsll((long long)leads) - 1];
+    const int id = sh.id[__ffs(leads) - 1];
     if (id < 0) {
       copy_rows(p, sh, row0, rank);
       continue;

@@ -9,7 +9,7 @@ namespace lora {
 
 constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 128;
-constexpr int MAX_TILE = 64;   // rows per tile, at most
+constexpr int MAX_TILE = 128;   // rows per tile, at most
 constexpr int NEAR = 64;       // adapters whose rank and scale every CTA reads
 
 struct LoraArgs {
@@ -25,7 +25,7 @@ struct LoraArgs {
 
 struct Tile {
   alignas(16) int32_t id[MAX_TILE];   // adapter of each row; -1: none; -2: past the last row
-  unsigned long long leads;  // rows that are the first of their adapter
+  uint32_t leads[MAX_TILE / 32];      // bits of the rows that are the first of their adapter
   // rank and scale of the first adapters, read beside the rows' indices rather than after them
   int32_t rank[NEAR];
   float scale[NEAR];
@@ -36,32 +36,30 @@ struct Adapter {
   float scale;
 };
 
-// The rows row0 .. row0 + rows - 1 by adapter (a multiple
-// of 4, <= MAX_TILE; at least 128 threads).  Rows without an adapter are a group of their own where `copies`.
-// An index past the last adapter is never followed: the row keeps its
-// projection, and the status says so where `report`.
+// The rows row0 .. row0 + rows - 1 by adapter (rows: a multiple of 4, at most
+// MAX_TILE; at least MAX_TILE + NEAR threads).  Rows without an adapter are a
+// group of their own where `copies`.  An index past the last adapter is never
+// followed: the row keeps its projection, and the status says so where `report`.
+// Ends with a barrier.
 __device__ __forceinline__ void group_rows(const LoraArgs& p, Tile& sh, int row0, int rows, bool report,
                                            bool copies) {
   const int tid = threadIdx.x;
-  if (tid == 0) sh.leads = 0;
-  if (tid >= 64 && tid < 64 + NEAR) {
-    const int a = tid - 64;
+  int id = -2;
+  if (tid < MAX_TILE) {
+    const int m = row0 + tid;
+    if (tid < rows && m < p.M) {
+      id = p.adapter[m];
+      if (id >= p.n_adapters && report) atomicExch(p.status, TSDS_E_INDEX);
+      if (id < 0 || id >= p.n_adapters) id = -1;
+    }
+    sh.id[tid] = id;
+  } else if (tid < MAX_TILE + NEAR) {
+    const int a = tid - MAX_TILE;
     sh.rank[a] = p.ranks && a < p.n_adapters ? p.ranks[a] : p.R;
     sh.scale[a] = p.scale && a < p.n_adapters ? p.scale[a] : 1.0f;
   }
-  if (tid < MAX_TILE) {
-    const int m = row0 + tid;
-    int id = tid < rows && m < p.M ? p.adapter[m] : -2;
-    if (tid < rows && m < p.M && id < 0) id = -1;
-    if (id >= p.n_adapters) {
-      id = -1;
-      if (report) atomicExch(p.status, TSDS_E_INDEX);
-    }
-    sh.id[tid] = id;
-  }
   __syncthreads();
-  if (tid < rows) {
-    const int id = sh.id[tid];
+  if (tid < MAX_TILE) {
     // without a branch: with one per row 64 rows took 3 us
     bool seen = false;
 #pragma unroll 4
@@ -70,7 +68,8 @@ __device__ __forceinline__ void group_rows(const LoraArgs& p, Tile& sh, int row0
       seen |= ((v.x == id) & (j < tid)) | ((v.y == id) & (j + 1 < tid)) | ((v.z == id) & (j + 2 < tid)) |
               ((v.w == id) & (j + 3 < tid));
     }
-    if (!seen && (id >= 0 || (id == -1 && copies))) atomicOr(&sh.leads, 1ull << tid);
+    const uint32_t bits = __ballot_sync(0xffffffffu, !seen && (id >= 0 || (id == -1 && copies)));
+    if ((tid & 31) == 0) sh.leads[tid >> 5] = bits;
   }
   __syncthreads();
 }

@@ -8,17 +8,18 @@
 //   through a TMA ring.  The partial sums meet over distributed shared memory
 //   (rank order: always the same bits), and t is stored as two bf16 words
 //   (hi + lo, 16 bits of it), so its rounding is far below the output's.
-// * expand: out = y + B t^T.  An item is 128 output channels x 64 token rows x
-//   adapter; two CTAs per SM share a block's items and take theirs in one
-//   sequence, with B and y of the next items on their way.  The products of
-//   both words of t go into one TMEM accumulator, two of which alternate, and
-//   each epilogue warp adds its 32 channels of 32 rows to y by itself.
+// * expand: out = y + B t^T.  A block is 128 token rows, which fill the MMA's M, so a
+//   lane of TMEM is a row; channels are its N.  The CTAs of a block take its channel
+//   tiles in turn: the y tile comes by TMA, the products of every adapter of the block
+//   (both words of t into one accumulator, two of which alternate) are added to
+//   their rows in shared memory, and the tile leaves by TMA once.
 //
 // The bytes of x and y bound both (B and A come from L2 after their first
 // use); the MMAs are a few percent of the tensor cores' rate.  2048 rows, K 5120,
-// rank 32 into q/k/v of 10240 columns: 36 us, shrink about 13 of them (21 MB of x, the
-// rest the chain from launch to reduction) and expand 21 (84 MB of y and out,
-// 4 TB/s).  Asking for y from shrink already, into L2, made it 43.
+// rank 32 into q/k/v of 10240 columns: 30.4 us, shrink about 13 of them (21 MB of x, the
+// rest the chain from launch to reduction) and expand 17 (84 MB of y and out,
+// 5 TB/s).  Asking for y from shrink already, into L2, cost 7 us.
+//
 // shrink lets its successor start only after its own dependency wait, so
 // everything before shrink is complete when expand begins, and expand may
 // read y, B and the indices before its wait; only t comes after it.
@@ -37,7 +38,7 @@ constexpr int CL = 8;               // CTAs per shrink cluster
 constexpr int THREADS = 192;        // TMA warp, MMA warp, four epilogue warps
 constexpr int BKE = 64;             // elements of K (or ranks) per block: a 128-byte swizzle row
 constexpr int RING = 8;             // most stages
-constexpr int A_SLACK = TILE_J * 128;   // the MMA reads 128 rows of A, a stage may hold fewer
+constexpr int SHRINK_SMEM = 110 * 1024;   // two CTAs per SM, with their static shared memory
 
 struct ShrinkArgs {
   LoraArgs l;
@@ -117,7 +118,10 @@ __global__ void __launch_bounds__(THREADS)
   group_rows(p.l, sh.tile, row0, p.nt, rank == 0 && slot == 0, false);
   tc_fence_after();   // (group_rows ends with a barrier)
   const uint32_t tmem = sh.tmem;
-  if (__popcll(sh.tile.leads) <= slot) {   // a cluster whose turn never comes
+  int adapters = 0;
+#pragma unroll
+  for (int w = 0; w < MAX_TILE / 32; ++w) adapters += __popc(sh.tile.leads[w]);
+  if (adapters <= slot) {   // a cluster whose turn never comes
     if (warp == 1) tmem_give(tmem, p.tmem_cols);
     return;
   }
@@ -127,10 +131,11 @@ __global__ void __launch_bounds__(THREADS)
   uint32_t phase = warp == 0 ? 1 : 0, tphase = 0;
   bool alive = true;
 
-  unsigned long long leads = sh.tile.leads;
-  for (int gi = 0; leads; ++gi, leads &= leads - 1) {
+  uint32_t leads = sh.tile.leads[0];
+  for (int gi = 0, word = 0; gi < adapters; ++gi, leads &= leads - 1) {
+    while (leads == 0) leads = sh.tile.leads[++word];
     if (gi % p.l.slots != slot) continue;
-    const Adapter ad = adapter_of(p.l, sh.tile, sh.tile.id[__ffsll((long long)leads) - 1]);
+    const Adapter ad = adapter_of(p.l, sh.tile, sh.tile.id[word * 32 + __ffs(leads) - 1]);
     const int ra16 = (ad.ra + 15) / 16 * 16;
     for (int u0 = 0; ad.ra > 0 && u0 < p.l.S * p.l.R; u0 += p.arows) {   // rank rows u0 .. u0 + arows - 1
       const bool all = ad.ra == p.l.R;
@@ -627,11 +632,11 @@ __global__ void __launch_bounds__(X_THREADS, PER_SM)
 int launch_shrink(const CUtensorMap& a_all, const CUtensorMap& a_box, const CUtensorMap& xmap, const ShrinkArgs& p,
                   cudaStream_t stream) {
   static tsds_device_flags limit_set;
-  const int st = tsds_smem_limit_once(shrink_kernel, 97 * 1024, limit_set);
+  const int st = tsds_smem_limit_once(shrink_kernel, SHRINK_SMEM, limit_set);
   if (st != TSDS_OK) return st;
-  // more of the SM's shared memory than of TMEM's columns (at least 57 KB for 64;
-  // expand: 200 KB for 256, 89 KB for 128), so CTAs that fit an SM never wait for columns
-  const int smem = p.stages * p.stage_bytes + A_SLACK + 1024;
+  // more of the SM's shared memory than of TMEM's columns (110 KB for up to 128; expand:
+  // 190 KB or more for 256, 89 KB or more for 128), so CTAs that fit an SM never wait for columns
+  const int smem = SHRINK_SMEM;
   tsds_launch_cluster(shrink_kernel, dim3((unsigned)(p.blocks * p.l.slots * CL)), dim3(THREADS), smem, stream, CL,
                       a_all, a_box, xmap, p);
   return tsds_launch_status();
@@ -664,15 +669,19 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.ld_t = l.S * p.Rp;
   // Token rows per shrink block: 32 for few rows (more clusters; 8 x 26 rows at
   // rank 64 into q/k/v 23.7 us, with 64 26.6), 64 above (an adapter's A is read
-  // less often; 16 x 26 rows, K 25600, rank 16 25.0 us, with 32 37.7)
-  p.nt = l.M <= 256 ? 32 : 64;
+  // less often; 16 x 26 rows, K 25600, rank 16 25.0 us, with 32 37.7), 128 where
+  // that still makes two CTAs per SM (4096 rows at rank 16 into q/k/v 47.5 us, with 64
+  // 52.6; 2048 rows at rank 32 32.3 and 30.5)
+  p.nt = l.M <= 256 ? 32 : (l.M < 3584 ? 64 : 128);
   p.blocks = (l.M + p.nt - 1) / p.nt;
   const int SR = l.S * l.R;
   p.arows = SR < TILE_J ? SR : TILE_J;
   p.bx = l.R % 16 ? 8 : 16;
   p.KT = (l.K + BKE - 1) / BKE;
   p.stage_bytes = (p.arows + p.nt) * 128;
-  p.stages = (96 * 1024 - A_SLACK) / p.stage_bytes;
+  // the MMA reads 128 rows from a stage's first, which may reach past its end
+  const int slack = p.arows + p.nt < TILE_J ? (TILE_J - p.arows - p.nt) * 128 : 0;
+  p.stages = (SHRINK_SMEM - 1024 - slack) / p.stage_bytes;
   if (p.stages > RING) p.stages = RING;
   p.tmem_cols = p.nt;
   p.idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.nt >> 3) << 17) | ((uint32_t)(TILE_J >> 4) << 24);
