@@ -54,7 +54,7 @@ constexpr int STAGING = 32 * TILE_J * 4;   // output staging of a persistent CTA
 constexpr int SMEM_SIDE = 2048;          // static shared memory + the system's 1 KB per CTA
 
 struct F8Args {
-  int M, n_out, KT, C, blocks;  // blocks of MAX_ROWS token rows
+  int M, n_out, KT, C, blocks, rows;  // blocks of token rows, rows of each but the last
   int units, bufs;              // units of the launch; accumulators per CTA
   int npad, stages, b_bytes, chunk;
   int out_off;                  // C == 1: offset of the output staging (0: the ring, free by then)
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
   // unit -> this CTA's weight tile and first token row; token blocks fastest, so
   // that the units in flight share their weights through L2
   auto tile_of = [&](int u) { return u / p.blocks * CG + half; };
-  auto row_of = [&](int u) { return (u - u / p.blocks * p.blocks) * MAX_ROWS; };
+  auto row_of = [&](int u) { return (u - u / p.blocks * p.blocks) * p.rows; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
     uint32_t tphase = 0;
     for (int u = first_unit; u < p.units; u += unit_step) {
       const Out w = out_of(tile_of(u), strip * 32, lane % 8, 8);
-      const int m0 = row_of(u), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+      const int m0 = row_of(u), rows = p.M - m0 < p.rows ? p.M - m0 : p.rows;
       prefetch_res(tile_of(u), m0, rows);
       const bool full = __all_sync(0xffffffffu, w.count == 4);
       struct Rows {   // what 32 rows take from global memory
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
   if constexpr (SPLIT) {
     pdl_wait();
     if (warp >= 2) {   // this CTA's share of the rows (of the first chunk)
-      const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+      const int m0 = row_of(first_unit), rows = p.M - m0 < p.rows ? p.M - m0 : p.rows;
       const int cn = rows < p.chunk ? rows : p.chunk, lo = rank * cn / p.C;
       prefetch_res(tile_of(first_unit), m0 + lo, (rank + 1) * cn / p.C - lo);
     }
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
     constexpr int G = SW ? 16 : 32, STEP = THREADS / G;
     const int g4 = threadIdx.x % G * 4;
     const Out w = out_of(tile_of(first_unit), 0, threadIdx.x % G, 1);
-    const int m0 = row_of(first_unit), rows = p.M - m0 < MAX_ROWS ? p.M - m0 : MAX_ROWS;
+    const int m0 = row_of(first_unit), rows = p.M - m0 < p.rows ? p.M - m0 : p.rows;
     for (int c0 = 0; c0 < rows; c0 += p.chunk) {
       const int cn = rows - c0 < p.chunk ? rows - c0 : p.chunk;
       if (alive && warp >= 2) {
@@ -603,6 +603,28 @@ Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas,
   return h;
 }
 
+// Token rows per block, a multiple of 32 above 256 rows.  Units that are all resident at once:
+// the fewest blocks, of even size.  Units in rounds: the size whose rounds, each
+// as long as its rows and the epilogue's share, take least; 2048 rows into 5120
+// (20 pairs of tiles) are 3 rounds of 74 units with blocks of 256 rows, and 3 rounds of three
+// quarters the length with blocks of 192.
+int block_rows(int M, int tiles) {
+  if (M <= MAX_ROWS) return MAX_ROWS;
+  const long long pairs = (tiles + 1) / 2, places = tsds_tc_num_sms() / 2;
+  const int fewest = (M + MAX_ROWS - 1) / MAX_ROWS;
+  if (pairs * fewest <= places) return ((M + fewest - 1) / fewest + 31) / 32 * 32;
+  int best = MAX_ROWS;
+  long long least = 0;
+  for (int r = MAX_ROWS; r >= TILE_J; r -= 32) {
+    const long long units = pairs * ((M + r - 1) / r), cost = (units + places - 1) / places * (r + 32);
+    if (least == 0 || cost < least) {
+      least = cost;
+      best = r;
+    }
+  }
+  return best;
+}
+
 template <int EPI, int CG, bool SPLIT>
 int launch(const CUtensorMap& amap, const CUtensorMap& bmap, const F8Args& p, unsigned grid, size_t smem,
            cudaStream_t stream) {
@@ -622,9 +644,10 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   constexpr bool SW = EPI == EPI_SWIGLU;
   const int tiles = SW ? (p.n_out + 63) / 64 : (p.n_out + TILE_J - 1) / TILE_J;
   p.KT = (K + KB - 1) / KB;
-  p.blocks = (p.M + MAX_ROWS - 1) / MAX_ROWS;
+  p.rows = block_rows(p.M, tiles);
+  p.blocks = (p.M + p.rows - 1) / p.rows;
   TSDS_RETURN_IF((long long)tiles * p.blocks > 0x3fffffffll, TSDS_E_UNSUPPORTED);
-  const int widest = p.M < MAX_ROWS ? p.M : MAX_ROWS;
+  const int widest = p.M < p.rows ? p.M : p.rows;
   p.npad = (widest + 15) / 16 * 16;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.npad) p.tmem_cols *= 2;
