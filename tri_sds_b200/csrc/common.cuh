@@ -110,6 +110,40 @@ static inline void tsds_launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3
   cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Clusters of `size` CTAs (at most 8) that the current device holds at once, or 0
+// where it does not say: a GPC's SMs are not a multiple of every size (148 SMs,
+// one CTA each: 33 clusters of 4, 15 of 8).  `known`: the caller's record for this
+// kernel and shared memory, whose limit has been raised before.
+typedef std::atomic<int> tsds_cluster_counts[TSDS_MAX_DEVICES][9];
+template <typename Kernel>
+static inline int tsds_resident_clusters(Kernel kernel, int threads, size_t smem, int size,
+                                         tsds_cluster_counts& known) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= TSDS_MAX_DEVICES) {
+    cudaGetLastError();
+    return 0;
+  }
+  int n = known[dev][size].load(std::memory_order_relaxed) - 1;   // 0: not asked yet
+  if (n >= 0) return n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  known[dev][size].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 namespace tsds {
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

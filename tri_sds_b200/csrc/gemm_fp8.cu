@@ -520,26 +520,52 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
       }
       cluster_barrier();
       if (alive && w.count > 0) {
-        // this CTA's token rows, from every CTA's partials in rank order
+        // this CTA's token rows, from every CTA's partials in rank order; of pairs
+        // so many rows at once that eight loads are on their way
         const int hi = (rank + 1) * cn / p.C;
-        for (int mc = rank * cn / p.C + (int)threadIdx.x / G; mc < hi; mc += STEP) {
-          const uint2 res = load_res(No(), w.vec, w, m0 + c0 + mc);
-          const float sx = p.sx[m0 + c0 + mc];
-          const uint32_t at = smem_u32(part + mc * TILE_J + g4);
-          float4 acc[2];
+        auto join = [&](auto at_once, auto most) {
+          constexpr int NR = decltype(at_once)::value, MC = decltype(most)::value;
+          for (int m1 = rank * cn / p.C + (int)threadIdx.x / G; m1 < hi; m1 += STEP * NR) {
+            uint2 res[NR];
+            float sx[NR];
+            float4 acc[NR][2];
 #pragma unroll
-          for (int h = 0; h < (SW ? 2 : 1); ++h) {
-            float4 f[MAX_C];
+            for (int r = 0; r < NR; ++r)
+              if (m1 + r * STEP < hi) {
+                res[r] = load_res(No(), w.vec, w, m0 + c0 + m1 + r * STEP);
+                sx[r] = p.sx[m0 + c0 + m1 + r * STEP];
+              }
 #pragma unroll
-            for (int q = 0; q < MAX_C; ++q)
-              if (q < p.C) f[q] = ld_peer(mapa_shared(at + h * 256, q * CG + half));
-            acc[h] = f[0];
+            for (int h = 0; h < (SW ? 2 : 1); ++h) {
+              float4 f[NR][MC];
 #pragma unroll
-            for (int q = 1; q < MAX_C; ++q)
-              if (q < p.C) acc[h] = add4(acc[h], f[q]);
+              for (int r = 0; r < NR; ++r) {
+                const uint32_t at = smem_u32(part + (m1 + r * STEP) * TILE_J + g4) + h * 256;
+#pragma unroll
+                for (int q = 0; q < MC; ++q)
+                  if (q < p.C && m1 + r * STEP < hi) f[r][q] = ld_peer(mapa_shared(at, q * CG + half));
+              }
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+                acc[r][h] = f[r][0];
+#pragma unroll
+                for (int q = 1; q < MC; ++q)
+                  if (q < p.C) acc[r][h] = add4(acc[r][h], f[r][q]);
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              if (m1 + r * STEP < hi) finish(No(), w.vec, w, m0 + c0 + m1 + r * STEP, acc[r], sx[r], res[r]);
           }
-          finish(No(), w.vec, w, m0 + c0 + mc, acc, sx, res);
-        }
+        };
+        // (of one-CTA units, which run up to three to an SM, one row: more would
+        // take the registers of the third)
+        if constexpr (CG == 1)
+          join(std::integral_constant<int, 1>(), std::integral_constant<int, MAX_C>());
+        else if (p.C <= 2)
+          join(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+        else
+          join(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
       }
       cluster_barrier();   // the peers are done with this CTA's partials
     }
@@ -561,19 +587,35 @@ struct Shape {
   int CG = 1, C = 1, stages = 0;
   bool persistent = false;
   long long grid = 0;
-  double cost = 1e30;   // estimated time, in units of its own
+  double cost = 1e30;   // estimated time, us
 };
+
+size_t smem_budget(int ctas) {
+  const int budget = SMEM_SM / ctas - SMEM_SIDE;
+  return budget < SMEM_CTA ? budget : SMEM_CTA;
+}
+
+// Clusters of `size` CTAs resident at once, `ctas` CTAs per SM.  Asked of a kernel
+// with the same threads and shared memory, never launched: of one that allocates
+// TMEM the runtime says one CTA per SM.
+__global__ void __launch_bounds__(THREADS) occupancy_kernel() {}
+int resident(int ctas, int size) {
+  static tsds_device_flags limit_set;
+  static tsds_cluster_counts known[3];
+  if (tsds_smem_limit_once(occupancy_kernel, SMEM_CTA, limit_set) != TSDS_OK) return 0;
+  return tsds_resident_clusters(occupancy_kernel, THREADS, smem_budget(ctas), size, known[ctas - 1]);
+}
 
 // What bounds the kernel up to 256 token rows is how many bytes of weights are
 // in flight: an SM holds a few hundred open requests, and a DRAM access
 // takes about a microsecond, so the rate grows with (CTAs x stages x 16 KB) up to
-// about 16 MB.  A launch whose units are all resident at once takes time
-// in inverse proportion to that.  One that is not goes in rounds, and its last
-// round lasts at least as long as one unit on one SM.  Measured: q/k/v
-// (80 units) at 26 rows 13.1 us on one CTA per SM (C = 1, 10 MB in flight),
-// 12.3 on two (C = 3, 16 MB and more); O (40 units) at 208 rows 22.1 us on one
-// (C = 3, 9.8 MB), 23.8 on two (C = 6, 7.8 MB); gate/up (400 units) at 128 rows
-// 49.7 us on one persistent CTA per SM, 60.4 on two.
+// about 16 MB: 0.4 bytes per us for each in flight.  A launch whose units are not
+// all resident at once goes in rounds, and its last round lasts at least as long
+// as one unit on one SM.  Joining the parts of a split unit takes a microsecond
+// and 20 ns per row.  Measured: q/k/v (80 tiles) at 26 rows 13.1 us on one CTA per
+// SM (C = 1, 10 MB in flight), 12.0 on two (C = 3, 16 MB and more); at 200 rows
+// (40 pairs) 18.2 on one (C = 1), 21.4 on two (C = 3); gate/up (400 tiles) at 128
+// rows 49.7 us on one persistent CTA per SM, 60.4 on two.
 Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas, int CG) {
   Shape h;
   h.CG = CG;
@@ -582,14 +624,16 @@ Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas,
   const long long places = (long long)sms * ctas / CG;   // units resident at once
   h.persistent = units > places;
   if (ctas * tmem_cols * (h.persistent ? 2 : 1) > 512) return h;
-  int budget = SMEM_SM / ctas - SMEM_SIDE;
-  if (budget > SMEM_CTA) budget = SMEM_CTA;
+  const int budget = (int)smem_budget(ctas);
   h.stages = (budget - 1024 - (h.persistent ? STAGING : 0)) / (A_BYTES + npad / CG * KB);
   if (h.stages > RING) h.stages = RING;
-  // K over as many CTAs as keep the whole launch resident, with a tenth of
-  // the places to spare: clusters do not fill a GPC's SMs exactly, and one
-  // that has to wait for a place doubles the time
-  while ((h.C + 1) * CG <= MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9) ++h.C;
+  // K over as many CTAs as keep the whole launch resident, with a tenth of the
+  // places to spare for the next one: a cluster that has to wait for a place
+  // doubles the time (26 rows, 6144 -> 2048: 12.5 us with 16 clusters of 8, of
+  // which 15 fit, 6.8 with 16 of 6)
+  while ((h.C + 1) * CG <= MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9 &&
+         units <= resident(ctas, (h.C + 1) * CG))
+    ++h.C;
   h.grid = h.persistent ? places : units * h.C;   // in units' CTAs, CG of them each
   double waste = 1.0;
   if (h.persistent) {
@@ -599,7 +643,9 @@ Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas,
   }
   double flight = (double)h.grid * CG * h.stages * A_BYTES;
   if (flight > 16e6) flight = 16e6;
-  h.cost = waste / flight;
+  const double bytes = (double)units * CG * KT * A_BYTES;
+  h.cost = waste * bytes / (0.4 * flight);   // us
+  if (h.C > 1) h.cost += 1 + 0.02 * (npad + h.C);
   return h;
 }
 

@@ -366,11 +366,26 @@ __global__ void __launch_bounds__(F::THREADS, F::CTAS) lora_kernel(LoraArgs p) {
   }
 }
 
+// shared memory of the largest call
+template <typename F>
+constexpr int most_smem() {
+  return F::WORK + 2 * TR * (RANKS + 16) * (int)sizeof(bf16);
+}
+
+// Clusters of the larger CTAs, one CTA per SM, that are resident at once.
+using Large = First<8, 2, 12, 1>;
+int resident_large() {
+  static tsds_device_flags limit_set;
+  static tsds_cluster_counts known;
+  if (tsds_smem_limit_once(lora_kernel<Large>, most_smem<Large>(), limit_set) != TSDS_OK) return 0;
+  return tsds_resident_clusters(lora_kernel<Large>, Large::THREADS, most_smem<Large>(), CL, known);
+}
+
 template <typename F>
 int launch_lora(LoraArgs p, cudaStream_t stream) {
   static tsds_device_flags limit_set;
   const int smem = F::WORK + 2 * TR * p.ld_t * (int)sizeof(bf16);
-  constexpr int most = F::WORK + 2 * TR * (RANKS + 16) * (int)sizeof(bf16);
+  constexpr int most = most_smem<F>();
   static_assert(most <= 226 * 1024, "shared memory of a CTA");
   const int st = tsds_smem_limit_once(lora_kernel<F>, most, limit_set);
   if (st != TSDS_OK) return st;
@@ -455,7 +470,7 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   // one-token requests 10.9 us, 14.2 with the smaller CTAs).  With more of them two
   // smaller CTAs per SM overlap (8 x 26 rows 14.3 us, 21.7 with the larger ones).
   const int most = (M + TR - 1) / TR * (n_adapters < TR ? n_adapters : TR);
-  if (most > tsds_tc_num_sms() / CL) return launch_lora<First<8, 1, 8, 2>>(p, stream);
+  if (most > resident_large()) return launch_lora<First<8, 1, 8, 2>>(p, stream);
   if (n_slices * R <= 16) return launch_lora<First<2, 4, 16, 1>>(p, stream);
-  return launch_lora<First<8, 2, 12, 1>>(p, stream);
+  return launch_lora<Large>(p, stream);
 }
