@@ -110,21 +110,28 @@ static inline void tsds_launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3
   cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// Clusters of `size` CTAs (at most 8) that the current device holds at once, or 0
+// The current device's index, or -1.
+static inline int tsds_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < TSDS_MAX_DEVICES) return dev;
+  cudaGetLastError();
+  return -1;
+}
+
+// Clusters of `size` CTAs (at most 8) that the current device `dev` holds at once, or 0
 // where it does not say: a GPC's SMs are not a multiple of every size (148 SMs,
 // one CTA each: 33 clusters of 4, 15 of 8).  `known`: the caller's record for this
-// kernel and shared memory, whose limit has been raised before.
+// kernel and shared memory.
 typedef std::atomic<int> tsds_cluster_counts[TSDS_MAX_DEVICES][9];
 template <typename Kernel>
-static inline int tsds_resident_clusters(Kernel kernel, int threads, size_t smem, int size,
+static inline int tsds_resident_clusters(int dev, Kernel kernel, int threads, size_t smem, int size,
                                          tsds_cluster_counts& known) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= TSDS_MAX_DEVICES) {
+  int n = known[dev][size].load(std::memory_order_relaxed) - 1;   // 0: not asked yet
+  if (n >= 0) return n;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  int n = known[dev][size].load(std::memory_order_relaxed) - 1;   // 0: not asked yet
-  if (n >= 0) return n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(size);
   cfg.blockDim = dim3(threads);

@@ -599,11 +599,9 @@ size_t smem_budget(int ctas) {
 // with the same threads and shared memory, never launched: of one that allocates
 // TMEM the runtime says one CTA per SM.
 __global__ void __launch_bounds__(THREADS) occupancy_kernel() {}
-int resident(int ctas, int size) {
-  static tsds_device_flags limit_set;
+int resident(int dev, int ctas, int size) {
   static tsds_cluster_counts known[3];
-  if (tsds_smem_limit_once(occupancy_kernel, SMEM_CTA, limit_set) != TSDS_OK) return 0;
-  return tsds_resident_clusters(occupancy_kernel, THREADS, smem_budget(ctas), size, known[ctas - 1]);
+  return tsds_resident_clusters(dev, occupancy_kernel, THREADS, smem_budget(ctas), size, known[ctas - 1]);
 }
 
 // What bounds the kernel up to 256 token rows is how many bytes of weights are
@@ -616,7 +614,7 @@ int resident(int ctas, int size) {
 // SM (C = 1, 10 MB in flight), 12.0 on two (C = 3, 16 MB and more); at 200 rows
 // (40 pairs) 18.2 on one (C = 1), 21.4 on two (C = 3); gate/up (400 tiles) at 128
 // rows 49.7 us on one persistent CTA per SM, 60.4 on two.
-Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas, int CG) {
+Shape shape_of(int dev, int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas, int CG) {
   Shape h;
   h.CG = CG;
   const int sms = tsds_tc_num_sms();
@@ -632,7 +630,7 @@ Shape shape_of(int tiles, int blocks, int KT, int npad, int tmem_cols, int ctas,
   // doubles the time (26 rows, 6144 -> 2048: 12.5 us with 16 clusters of 8, of
   // which 15 fit, 6.8 with 16 of 6)
   while ((h.C + 1) * CG <= MAX_C && KT >= 2 * (h.C + 1) && units * (h.C + 1) * 10 <= places * 9 &&
-         units <= resident(ctas, (h.C + 1) * CG))
+         units <= resident(dev, ctas, (h.C + 1) * CG))
     ++h.C;
   h.grid = h.persistent ? places : units * h.C;   // in units' CTAs, CG of them each
   double waste = 1.0;
@@ -697,10 +695,12 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   p.npad = (widest + 15) / 16 * 16;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.npad) p.tmem_cols *= 2;
+  const int dev = tsds_device();
+  TSDS_RETURN_IF(dev < 0, TSDS_E_DEVICE);
   Shape best;
   for (int CG = 1; CG <= (p.npad > TILE_J ? 2 : 1); ++CG)
     for (int ctas = 1; ctas <= 3; ++ctas) {
-      const Shape h = shape_of(tiles, p.blocks, p.KT, p.npad, p.tmem_cols, ctas, CG);
+      const Shape h = shape_of(dev, tiles, p.blocks, p.KT, p.npad, p.tmem_cols, ctas, CG);
       if (h.stages >= 2 && h.cost <= best.cost) best = h;
     }
   TSDS_RETURN_IF(best.stages < 2, TSDS_E_UNSUPPORTED);

@@ -44,12 +44,12 @@ constexpr int RANKS = 64;     // columns of t, at most: 8 n8 tiles
 // the rows' bytes and the (tile, adapter) pairs decide; how many pairs occur is known
 // only up to tiles x min(adapters, 16).  Measured, here and there (K 5120 into
 // q/k/v of 10240, or K 8192 -> 5120): 8 rows of 8 adapters, rank 16 in three slices
-// 10.9 and 15.0 us, rank 32 in three 16.7 and 15.6, rank 64 in one 13.6 and 15.2; 32
-// rows, rank 64 in one 13.3 and 12.5; 8 x 26 rows, rank 16 in three 14.3 and 15.8, rank
-// 32 in three 22.4 and 16.6; 512 rows of one adapter, rank 16 in three 15.1 and 16.8,
-// rank 16 in one 12.5 and 15.0, 1024 rows 23.6 and 18.4; 128 rows that alternate
-// between 16 adapters, rank 16 in one 45 and 28.  K 25600 -> 5120: 512 rows, rank
-// 64 43 and 22.8; 208 rows, rank 16 19.3 and 20.9.
+// 10.8 and 14.9 us, rank 64 in one 13.1 and 15.2; 32 rows, rank 64 in one 13.0 and
+// 13.4; 8 x 26 rows, rank 16 in three 14.8 and 15.9, rank 32 in one 14.0 and 14.2; 512
+// rows of one adapter, rank 16 in three 15.2 and 15.5, rank 16 in one 13.1 and 13.7, rank
+// 32 in one 16.7 and 14.1, 1024 rows 24.2 and 18.4; 128 rows that alternate between 16
+// adapters, rank 16 in one 44 and 29.  K 25600 -> 5120: 8 rows, rank 16 10.3 and 21.3;
+// 208 rows, rank 48 28.8 and 21.3; 512 rows, rank 64 42.8 and 21.3.
 bool few_rows(int M, int K, int R, int S, int n_adapters) {
   const int tiles = (M + TR - 1) / TR, SR = S * R;
   if (M > 512 || tiles * (n_adapters < TR ? n_adapters : TR) > 104) return false;
@@ -375,10 +375,9 @@ constexpr int most_smem() {
 // Clusters of the larger CTAs, one CTA per SM, that are resident at once.
 using Large = First<8, 2, 12, 1>;
 int resident_large() {
-  static tsds_device_flags limit_set;
   static tsds_cluster_counts known;
-  if (tsds_smem_limit_once(lora_kernel<Large>, most_smem<Large>(), limit_set) != TSDS_OK) return 0;
-  return tsds_resident_clusters(lora_kernel<Large>, Large::THREADS, most_smem<Large>(), CL, known);
+  const int dev = tsds_device();
+  return dev < 0 ? 0 : tsds_resident_clusters(dev, lora_kernel<Large>, Large::THREADS, most_smem<Large>(), CL, known);
 }
 
 template <typename F>
@@ -467,8 +466,8 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   }
   // Where a cluster for every adapter of every tile fits the SMs at once the call
   // is a matter of latency: many warps and loads per CTA (q/k/v adapters of 8
-  // one-token requests 10.9 us, 14.2 with the smaller CTAs).  With more of them two
-  // smaller CTAs per SM overlap (8 x 26 rows 14.3 us, 21.7 with the larger ones).
+  // one-token requests 10.8 us, 14.2 with the smaller CTAs).  With more of them two
+  // smaller CTAs per SM overlap (8 x 26 rows 14.8 us, 21.7 with the larger ones).
   const int most = (M + TR - 1) / TR * (n_adapters < TR ? n_adapters : TR);
   if (most > resident_large()) return launch_lora<First<8, 1, 8, 2>>(p, stream);
   if (n_slices * R <= 16) return launch_lora<First<2, 4, 16, 1>>(p, stream);

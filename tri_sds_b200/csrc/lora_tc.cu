@@ -668,10 +668,10 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.Rp = rank_columns(l.R);
   p.ld_t = l.S * p.Rp;
   // Token rows per shrink block: 32 for few rows (more clusters; 8 x 26 rows at
-  // rank 64 into q/k/v 23.7 us, with 64 26.6), 64 above (an adapter's A is read
-  // less often; 16 x 26 rows, K 25600, rank 16 25.0 us, with 32 37.7), 128 where
-  // that still makes two CTAs per SM (4096 rows at rank 16 into q/k/v 47.5 us, with 64
-  // 52.6; 2048 rows at rank 32 32.3 and 30.5)
+  // rank 64 into q/k/v 23.6 us, with 64 26.2), 64 above (an adapter's A is read
+  // less often; 16 x 26 rows, K 25600, rank 16 26 us, with 32 37), 128 where
+  // that still makes two CTAs per SM (4096 rows at rank 16 into q/k/v 47.7 us, with 64
+  // 52.7; 2048 rows at rank 32 32.3 and 30.4)
   p.nt = l.M <= 256 ? 32 : (l.M < 3584 ? 64 : 128);
   p.blocks = (l.M + p.nt - 1) / p.nt;
   const int SR = l.S * l.R;
@@ -689,7 +689,7 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   // A cluster per adapter of a block of rows as long as all are resident at
   // once; beyond that each takes several in turn.  One without an adapter
   // holds the next launch up: with twice as many the q/k/v adapters of 256 rows
-  // that alternate between 8 adapters of rank 64 take 47 us instead of 44.
+  // that alternate between 8 adapters of rank 64 take 43.5 us instead of 40.9.
   const int sms = tsds_tc_num_sms();
   p.l.slots = 2 * sms / CL / p.blocks;
   p.l.slots = p.l.slots < 1 ? 1 : (p.l.slots > p.nt ? p.nt : p.l.slots);
