@@ -647,22 +647,24 @@ Shape shape_of(int dev, int tiles, int blocks, int KT, int npad, int tmem_cols, 
   return h;
 }
 
-// Token rows per block, a multiple of 32 above 256 rows.  Units that are all resident at once:
-// the fewest blocks, of even size.  Units in rounds: the size whose rounds, each
-// as long as its rows and the epilogue's share, take least; 2048 rows into 5120
-// (20 pairs of tiles) are 3 rounds of 74 units with blocks of 256 rows, and 3 rounds of three
-// quarters the length with blocks of 192.
-int block_rows(int M, int tiles) {
+// Token rows per block, a multiple of 32 above 256 rows: what takes least by this
+// estimate, 0.34 us for a block of K and 256 rows on a pair of CTAs, the epilogue's share of
+// 32 rows, units in rounds or, all resident, their K over several pairs, whose
+// parts then have to be joined.  2048 rows into 5120 (20 pairs of tiles) are 3 rounds of 74
+// units with blocks of 256 rows, and 3 rounds of three quarters the length with
+// blocks of 192.
+int block_rows(int M, int tiles, int KT) {
   if (M <= MAX_ROWS) return MAX_ROWS;
   const long long pairs = (tiles + 1) / 2, places = tsds_tc_num_sms() / 2;
-  const int fewest = (M + MAX_ROWS - 1) / MAX_ROWS;
-  if (pairs * fewest <= places) return ((M + fewest - 1) / fewest + 31) / 32 * 32;
   int best = MAX_ROWS;
-  long long least = 0;
-  for (int r = MAX_ROWS; r >= TILE_J; r -= 32) {
-    const long long units = pairs * ((M + r - 1) / r), cost = (units + places - 1) / places * (r + 32);
-    if (least == 0 || cost < least) {
-      least = cost;
+  double least = 0;
+  for (int r = MAX_ROWS; r > TILE_J; r -= 32) {   // (128 rows and fewer are not for pairs)
+    const long long units = pairs * ((M + r - 1) / r), rounds = (units + places - 1) / places;
+    long long C = places * 9 / (units * 10);
+    C = C < 1 ? 1 : (C > MAX_C / 2 ? MAX_C / 2 : C);
+    const double t = rounds * (r + 32) * KT * (0.34 / 256) / C + (C > 1 ? 1 + 0.02 * r : 0);
+    if (least == 0 || t < least) {
+      least = t;
       best = r;
     }
   }
@@ -688,7 +690,7 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
   constexpr bool SW = EPI == EPI_SWIGLU;
   const int tiles = SW ? (p.n_out + 63) / 64 : (p.n_out + TILE_J - 1) / TILE_J;
   p.KT = (K + KB - 1) / KB;
-  p.rows = block_rows(p.M, tiles);
+  p.rows = block_rows(p.M, tiles, p.KT);
   p.blocks = (p.M + p.rows - 1) / p.rows;
   TSDS_RETURN_IF((long long)tiles * p.blocks > 0x3fffffffll, TSDS_E_UNSUPPORTED);
   const int widest = p.M < p.rows ? p.M : p.rows;
