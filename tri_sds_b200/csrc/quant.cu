@@ -15,6 +15,11 @@
 // exact arithmetic, instead of to the side that the scale's rounding picks.
 // Sums and maxima are fp32; max.NaN keeps a NaN, so a row that holds one
 // gets a NaN scale and NaN values.
+//
+// A row stays in one CTA's registers, so each of its bytes moves once and HBM
+// bounds many rows: 10240 rows of 5120 quantised in 25.4 us (6.2 TB/s), 4096 rows
+// of 5120 with residual, norm and both outputs in 29.9 us (6.3 TB/s).  Few rows are a
+// launch, the row's loads and the CTA's two reductions: 26 rows of 25600 in 2.8 us.
 #include "common.cuh"
 #include "linear.cuh"
 
@@ -214,7 +219,9 @@ int launch(const QuantArgs& a, int rows, cudaStream_t stream) {
 // Rows of up to 8192 elements: 256 threads.  Longer ones: 1024 threads where
 // the rows are few and one row's time is what counts; with many rows half as
 // many threads with twice the vectors each keep more loads in flight per SM
-// (quantising 5809 rows of 9024: 55 us with 1024 threads).
+// (quantising 5809 rows of 9024: 28.8 us, 55 with 1024 threads).  The threads set the
+// order in which a norm's squares are summed, so above 8192 elements a row's last
+// bits may differ between calls of few and of many rows.
 template <bool NORM>
 int launch_rows(const QuantArgs& a, int rows, cudaStream_t stream) {
   if (a.n <= 8192) return launch<NORM, 256, 4>(a, rows, stream);
