@@ -1,0 +1,62 @@
+"""GPU checks of the 8-bit operators where numbers, sizes or orders of work are extreme."""
+import pytest
+import torch
+
+import fp8_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from tri_sds_b200 import ops as o
+    yield o
+    o.check_status()
+
+
+def _norm_values(x, w, eps):
+    r = x.double()
+    return r / torch.sqrt(r.square().mean(dim=1, keepdim=True) + eps) * w.double()
+
+
+@pytest.mark.parametrize("n", [512, 40000])
+@pytest.mark.parametrize("eps", [1e-6, 1e-12, 1e-20, 1e-38])
+def test_norm_of_zero_rows_with_a_small_eps(ops, n, eps):
+    """A padding row is zeros whatever eps lifts it by."""
+    x = torch.randn(5, n, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n)).to(BF)
+    x[1] = x[3] = 0
+    w = torch.ones(n, device=DEV, dtype=BF)
+    no = torch.empty_like(x)
+    q, s, _ = ops.add_rms_norm_fp8(x, w, eps=eps, norm_out=no)
+    for row in (1, 3):
+        assert (q[row].float() == 0).all() and (no[row] == 0).all()
+        assert abs(s[row].double().item() / (ref.TINY / ref.TOP) - 1) < 1e-6
+    assert torch.isfinite(q.float()).all() and torch.isfinite(s).all()
+
+
+# The root's relative error is half of the sum's: at n = 512 (64 threads with a vector of 8, 8 warps) at
+# most 8 + 5 + 8 additions, so 11 of 2^-24, then the mean, eps, root, reciprocal, the product with the largest value and
+# the multiplier: 20 of 2^-24 in all.
+RSTD = 20 * ref.F32
+
+
+@pytest.mark.parametrize("eps,x_exp,w_exp", [(1e-12, -70, -45), (1e-12, -60, -59), (1e-14, -61, -60), (1e-14, -63, -62),
+                                             (1e-20, -60, -55), (1e-20, -80, -46), (1e-6, -100, 0), (1e-12, -118, 2)])
+def test_norm_of_tiny_rows_with_a_small_eps(ops, eps, x_exp, w_exp):
+    """Values around the smallest magnitude a row is scaled to, lifted there by the norm alone."""
+    g = torch.Generator(device=DEV).manual_seed(-x_exp)
+    n = 512
+    x = (torch.ldexp(torch.rand(4, n, device=DEV, generator=g, dtype=torch.float64) - 0.5,
+                     torch.tensor(x_exp, device=DEV))).to(BF)
+    w = torch.ldexp(torch.rand(n, device=DEV, generator=g, dtype=torch.float64) + 0.5,
+                    torch.tensor(w_exp, device=DEV)).to(BF)
+    q, s, _ = ops.add_rms_norm_fp8(x, w, eps=eps)
+    v, s_ref = ref.quant(_norm_values(x, w, eps))
+    assert ((s.double() - s_ref).abs() <= s_ref * RSTD).all()
+    # (products below 2^-126 keep at least 2^-149; the largest here are above 2^-130)
+    lim = ref.e4m3_step(v) / 2 + v.abs() * RSTD + ref.TOP * 2.0 ** -19
+    off = (q.double() - v).abs()
+    assert (off <= lim).all(), (off - lim).max()

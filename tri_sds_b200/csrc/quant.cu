@@ -29,6 +29,8 @@ namespace {
 
 constexpr float kTop = 448.0f;              // largest e4m3 value
 constexpr float kTiny = 7.88860905e-31f;    // 2^-100: smallest magnitude a row is scaled to
+constexpr float kSmall = 8.67361738e-19f;   // 2^-60: products below it are moved up first,
+constexpr float kUp = 1.84467441e19f;       // by 2^64
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -82,11 +84,11 @@ __device__ __forceinline__ void reduce8(uint4 r, uint4 g, float& sum, float& top
   }
 }
 
-// eight elements quantised (hi + lo: the two words of the multiplier), and
-// with norm_out their normed values (r * rstd) * w rounded to bf16
+// eight elements times the row's power of two quantised (hi + lo: the two words of the
+// multiplier), and with norm_out their normed values (r * rstd) * w rounded to bf16
 template <bool NORM>
-__device__ __forceinline__ void store8(const QuantArgs& a, uint8_t* qrow, bf16* nrow, int c, uint4 r, uint4 g, float hi,
-                                       float lo, float rstd) {
+__device__ __forceinline__ void store8(const QuantArgs& a, uint8_t* qrow, bf16* nrow, int c, uint4 r, uint4 g, float pre,
+                                       float hi, float lo, float rstd) {
   const uint32_t u[4] = {r.x, r.y, r.z, r.w}, w[4] = {g.x, g.y, g.z, g.w};
   uint32_t h[4];
 #pragma unroll
@@ -95,6 +97,8 @@ __device__ __forceinline__ void store8(const QuantArgs& a, uint8_t* qrow, bf16* 
     if constexpr (NORM) {
       p0 *= bf_lo(w[i]);
       p1 *= bf_hi(w[i]);
+      p0 *= pre;
+      p1 *= pre;
     }
     h[i] = pack_e4m3x2(fmaf(p0, hi, p0 * lo), fmaf(p1, hi, p1 * lo));
   }
@@ -187,25 +191,30 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
   }
   const float rstd = NORM ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
   const float amax = rstd * top;
+  // Where rstd lifts a row of tiny products the multiplier could pass the largest fp32
+  // number (a row of zeros with eps = 1e-12: 0 * inf): the products are
+  // moved up by a power of two, exactly, and the multiplier is as much smaller.
+  const float pre = NORM && top < kSmall ? kUp : 1.0f;
   float hi, lo = 0.f;
   if (amax >= kTiny) {
-    hi = kTop / top;
-    lo = fmaf(-hi, top, kTop) / top;
+    const float m = top * pre;
+    hi = kTop / m;
+    lo = fmaf(-hi, m, kTop) / m;
   } else {  // an (almost) empty row, or a NaN
-    hi = amax != amax ? amax : rstd * (kTop / kTiny);
+    hi = amax != amax ? amax : rstd * (kTop / kTiny / pre);
   }
   if (t == 0) a.scale[row] = (amax < kTiny ? kTiny : amax) / kTop;
   if (keep) {
 #pragma unroll
     for (int i = 0; i < VMAX; ++i) {
       const int c = t + i * NT;
-      if (c < nv) store8<NORM>(a, qr, nr, c, v[i], g[i], hi, lo, rstd);
+      if (c < nv) store8<NORM>(a, qr, nr, c, v[i], g[i], pre, hi, lo, rstd);
     }
   } else {
     const bf16* src = NORM && rr ? ro : xr;
     for (int c = t; c < nv; c += NT) {
       const uint4 w = NORM ? ldg16(a.w + c * 8) : make_uint4(0, 0, 0, 0);
-      store8<NORM>(a, qr, nr, c, ld16(src + c * 8), w, hi, lo, rstd);
+      store8<NORM>(a, qr, nr, c, ld16(src + c * 8), w, pre, hi, lo, rstd);
     }
   }
 }
