@@ -60,3 +60,33 @@ def test_norm_of_tiny_rows_with_a_small_eps(ops, eps, x_exp, w_exp):
     lim = ref.e4m3_step(v) / 2 + v.abs() * RSTD + ref.TOP * 2.0 ** -19
     off = (q.double() - v).abs()
     assert (off <= lim).all(), (off - lim).max()
+
+
+def test_norm_weights_made_just_before_the_call(ops):
+    """The norm may start while the kernel that makes its weights still runs: they are read after it."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    n = 5120
+    x = torch.randn(4, n, device=DEV, generator=g).to(BF)
+    gammas = [torch.randn(n, device=DEV, generator=g).to(BF) for _ in range(4)]
+    wq, ws = ops.quant_fp8(torch.randn(n, n, device=DEV, generator=g).to(BF))
+    xq, xs = ops.quant_fp8(x)
+    w = torch.empty(n, device=DEV, dtype=BF)
+    outs = []
+    for i in range(40):
+        ops.linear_fp8(xq, xs, wq, ws)            # keeps the stream busy
+        torch.add(gammas[i % 4], 1.0, out=w)
+        outs.append(ops.add_rms_norm_fp8(x, w))
+    # the weights from a kernel of the library, which lets its successor start at once
+    made = [ops.rms_norm(gammas[i][None], gammas[i])[0].clone() for i in range(4)]
+    torch.cuda.synchronize()
+    late = []
+    for i in range(40):
+        ops.rms_norm(gammas[i % 4][None], gammas[i % 4], out=w[None])
+        late.append(ops.add_rms_norm_fp8(x, w))
+    torch.cuda.synchronize()
+    for i in range(4):
+        for weights, got in (((gammas[i] + 1.0), outs[i::4]), (made[i], late[i::4])):
+            q, s, _ = ops.add_rms_norm_fp8(x, weights.clone())
+            torch.cuda.synchronize()
+            for gq, gs, _ in got:
+                assert torch.equal(gq.view(torch.uint8), q.view(torch.uint8)) and torch.equal(gs, s)

@@ -130,13 +130,8 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
   bf16* nr = a.norm_out ? a.norm_out + row * a.ld_norm : nullptr;
   const bool keep = nv <= NT * VMAX;
   uint4 v[VMAX], g[VMAX];
-  if constexpr (NORM) {  // the norm's weights are constant: read before the wait
-#pragma unroll
-    for (int i = 0; i < VMAX; ++i) {
-      g[i] = make_uint4(0, 0, 0, 0);
-      if (keep && t + i * NT < nv) g[i] = ldg16(a.w + (t + i * NT) * 8);
-    }
-  }
+  // the weights too may come from the kernel before (1 + gamma, say), so nothing is read
+  // earlier, and by plain loads: 4.18 us instead of 4.10 at 208 rows of 5120
   pdl_wait();
   float sum = 0.f, top = 0.f;
   if (keep) {
@@ -146,6 +141,7 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
       const int c = t + i * NT;
       v[i] = c < nv ? ld16(xr + c * 8) : make_uint4(0, 0, 0, 0);
       if (NORM && rr && c < nv) b[i] = ld16(rr + c * 8);
+      if constexpr (NORM) g[i] = c < nv ? ld16(a.w + c * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < VMAX; ++i) {
@@ -163,7 +159,7 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
       uint4 r = ld16(xr + c * 8);
       uint4 w = make_uint4(0, 0, 0, 0);
       if constexpr (NORM) {
-        w = ldg16(a.w + c * 8);
+        w = ld16(a.w + c * 8);
         if (rr) {
           r = add8(r, ld16(rr + c * 8));
           *reinterpret_cast<uint4*>(ro + c * 8) = r;
@@ -213,7 +209,7 @@ __global__ void __launch_bounds__(NT) quant_rows_kernel(QuantArgs a) {
   } else {
     const bf16* src = NORM && rr ? ro : xr;
     for (int c = t; c < nv; c += NT) {
-      const uint4 w = NORM ? ldg16(a.w + c * 8) : make_uint4(0, 0, 0, 0);
+      const uint4 w = NORM ? ld16(a.w + c * 8) : make_uint4(0, 0, 0, 0);
       store8<NORM>(a, qr, nr, c, ld16(src + c * 8), w, pre, hi, lo, rstd);
     }
   }
