@@ -66,6 +66,8 @@ __device__ __forceinline__ void st_peer8(uint32_t addr, uint32_t a, uint32_t b) 
   asm volatile("st.shared::cluster.v2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 
+// (a plain load for A and B too: an adapter's may have been written by the kernel before,
+// whose end this one waits for after its own start)
 __device__ __forceinline__ uint4 ld16(const bf16* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // `bytes` (a multiple of 16) from a 16-byte aligned address into L2
@@ -187,7 +189,7 @@ __device__ __forceinline__ void expand(const LoraArgs& p, const Tile& sh, const 
         for (int i = 0; i < 4; ++i) {
           bv[c][i] = make_uint2(0, 0);
           if (col < p.N && left > 0)
-            bv[c][i] = __ldg(reinterpret_cast<const uint2*>(b_col + 2 * i * p.R + (c0 + c) * 16));
+            bv[c][i] = *reinterpret_cast<const uint2*>(b_col + 2 * i * p.R + (c0 + c) * 16);
         }
       }
 #pragma unroll
@@ -277,7 +279,7 @@ struct First {
         const bool in = c < hi && k + 8 * q < p.K;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-          av[u][i] = in && ar[i] >= 0 ? ldg16(a_id + (int64_t)ar[i] * p.K + k) : make_uint4(0, 0, 0, 0);
+          av[u][i] = in && ar[i] >= 0 ? ld16(a_id + (int64_t)ar[i] * p.K + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           xv[u][h] = in && row0 + g + 8 * h < p.M ? ld16(x_row + 8 * h * p.ldx + k) : make_uint4(0, 0, 0, 0);
