@@ -265,7 +265,9 @@ int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const v
  * 3): slice_widths (host array, each a multiple of 32, summing to N) gives
  * the columns of each, s(j) is column j's; NULL with one slice.  scale
  * (fp32) and ranks (int32, what an adapter uses of R; the rest of its A and
- * B is not part of the sum, whatever it holds) may be NULL: 1 and R.
+ * B is not part of the sum, whatever it holds) may be NULL: 1 and R.  The inner sum
+ * is held as two bf16 words, infinities as they are; an infinity in B itself can
+ * make a NaN of what the formula calls an infinity.
  * out may be y (ldo == ldy; rows without an adapter are then not touched),
  * not x.  Beyond a few rows n_adapters * N < 2^31.
  * Any order of adapters; rows of one request next to one another are

@@ -1,6 +1,9 @@
-"""GPU checks of the per-request adapters at the ends of their ranges."""
+"""GPU checks of the per-request adapters at the ends of their ranges: infinities, numbers at bf16's end,
+adapters that change between calls."""
 import pytest
 import torch
+
+import fp8_ref as ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -25,6 +28,54 @@ def _case(M, R, used, seed=0, K=264, slices=(96, 160), n_ad=3):
                 adapter=torch.tensor([m % (n_ad + 1) - 1 for m in range(M)], dtype=torch.int32, device=DEV),
                 scale=torch.rand(n_ad, device=DEV, generator=g) + 0.5,
                 ranks=torch.full((n_ad,), used, dtype=torch.int32, device=DEV), slices=list(slices))
+
+
+def _check(ops, st):
+    want, err = ref.lora(st["y"], st["x"], st["lora_a"], st["lora_b"], st["adapter"], st["scale"], st["ranks"], st["slices"])
+    got = ops.lora_add(**st)
+    fin = torch.isfinite(want)
+    assert not fin.all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(got.double()[inf], want[inf])
+    ref.check_bf16(got[fin], want[fin], err[fin])
+
+
+# one launch and two; ranks that end inside and at the end of 8 and 16
+SIZES = [(M, R, used) for M in (7, 40, 600, 1100) for R, used in ((8, 1), (16, 1), (16, 2), (24, 9), (64, 64), (128, 65))]
+
+
+@pytest.mark.parametrize("M,R,used", SIZES)
+def test_infinite_activation(ops, M, R, used):
+    st = _case(M, R, used)
+    st["x"][2, 100] = float("inf")
+    st["x"][5, 263] = float("-inf")
+    _check(ops, st)
+
+
+@pytest.mark.parametrize("M,R,used", SIZES)
+def test_infinite_scale_and_first_matrix(ops, M, R, used):
+    st = _case(M, R, used, seed=1)
+    st["scale"][1] = float("inf")
+    st["lora_a"][2, 0, 17] = float("-inf")
+    _check(ops, st)
+
+
+@pytest.mark.parametrize("M,R", [(7, 8), (40, 64), (600, 24), (1100, 128)])
+def test_first_product_between_the_largest_bf16_and_fp32(ops, M, R):
+    """A first product that bf16 would round to an infinity: its two words still hold it."""
+    st = _case(M, R, 1, seed=2)
+    st["x"].zero_()
+    st["lora_a"].zero_()
+    st["lora_b"].fill_(2.0 ** -20)
+    st["x"][:, 3] = 2.0 ** 64
+    for s in range(2):
+        st["lora_a"][:, s * R, 3] = 255 * 2.0 ** 56        # t = 255/256 2^128
+    st["scale"][:] = 1 + 511 * 2.0 ** -17                  # times that: below 2^128 in fp32, 2^128 in bf16
+    t = (torch.tensor(255 * 2.0 ** 120, device=DEV) * st["scale"][0])
+    assert torch.isfinite(t) and torch.isinf(t.to(BF))
+    want, err = ref.lora(st["y"], st["x"], st["lora_a"], st["lora_b"], st["adapter"], st["scale"], st["ranks"], st["slices"])
+    ref.check_bf16(ops.lora_add(**st), want, err)
 
 
 @pytest.mark.parametrize("M", [4, 40, 400, 1200])

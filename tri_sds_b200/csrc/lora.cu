@@ -135,12 +135,14 @@ __device__ __forceinline__ void exchange(const LoraArgs& p, const Ranks& ad, flo
     for (int k = 1; k < CL; ++k) s = make_float4(s.x + f[k].x, s.y + f[k].y, s.z + f[k].z, s.w + f[k].w);
     const int ti = c4 / 2, sl = ti / ad.nr8;
     const int to = m * p.ld_t + sl * ad.Rp + (ti - sl * ad.nr8) * 8 + (c4 & 1) * 4;
-    const float v[4] = {s.x * ad.scale, s.y * ad.scale, s.z * ad.scale, s.w * ad.scale};
-    float h[4];
+    // ranks past the adapter's are zeros: an infinite x or scale would make NaN of them
+    const int left = ad.ra - (ti - sl * ad.nr8) * 8 - (c4 & 1) * 4;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    float h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = rbf(v[k]);
+    for (int k = 0; k < 4; ++k) two_words(k < left ? v[k] * ad.scale : 0.f, h[k], l[k]);
     const uint32_t h0 = pack_bf2(h[0], h[1]), h1 = pack_bf2(h[2], h[3]);
-    const uint32_t l0 = pack_bf2(v[0] - h[0], v[1] - h[1]), l1 = pack_bf2(v[2] - h[2], v[3] - h[3]);
+    const uint32_t l0 = pack_bf2(l[0], l[1]), l1 = pack_bf2(l[2], l[3]);
     const uint32_t ah = smem_u32(t_hi + to), al = smem_u32(t_lo + to);
 #pragma unroll
     for (int k = 0; k < CL; ++k) {

@@ -88,6 +88,20 @@ __device__ __forceinline__ Adapter adapter_of(const LoraArgs& p, const Tile& sh,
   return ad;
 }
 
+// v as the sum of two bf16 words.  An infinity is in the first alone (its
+// remainder would be a NaN), and a number that bf16 would round to one has the largest
+// bf16 there and the rest in the second.
+__device__ __forceinline__ void two_words(float v, float& hi, float& lo) {
+  constexpr float most = 3.38953139e38f;   // the largest bf16
+  hi = rbf(v);
+  lo = v - hi;
+  if (fabsf(hi) > most) {
+    const bool inf = fabsf(v) > 3.40282347e38f;
+    hi = inf ? v : copysignf(most, v);
+    lo = inf ? 0.f : v - hi;
+  }
+}
+
 }  // namespace lora
 }  // namespace tsds
 

@@ -245,13 +245,13 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = r + k < ad.ra ? w[k] * ad.scale : 0.f;
         }
-        float h[4];
+        float h[4], l[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = rbf(v[k]);
+        for (int k = 0; k < 4; ++k) two_words(v[k], h[k], l[k]);
         bf16* to = p.t + (int64_t)(row0 + i) * 2 * p.ld_t + sl * p.Rp + r;
         *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf2(h[0], h[1]), pack_bf2(h[2], h[3]));
         *reinterpret_cast<uint2*>(to + p.ld_t) =
-            make_uint2(pack_bf2(v[0] - h[0], v[1] - h[1]), pack_bf2(v[2] - h[2], v[3] - h[3]));
+            make_uint2(pack_bf2(l[0], l[1]), pack_bf2(l[2], l[3]));
       }
       // the peers are done with this CTA's partials; the ring may be loaded again
       fence_proxy_async();
