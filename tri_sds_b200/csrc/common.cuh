@@ -121,13 +121,16 @@ static inline int tsds_device() {
 // Clusters of `size` CTAs (at most 8) that the current device `dev` holds at once, or 0
 // where it does not say: a GPC's SMs are not a multiple of every size (148 SMs,
 // one CTA each: 33 clusters of 4, 15 of 8).  `known`: the caller's record for this
-// kernel and shared memory.
+// kernel and shared memory; an answer is kept, a query that failed is not.  One kernel may be
+// asked about with several sizes of shared memory, so its limit is set and used under
+// the lock.
 typedef std::atomic<int> tsds_cluster_counts[TSDS_MAX_DEVICES][9];
 template <typename Kernel>
 static inline int tsds_resident_clusters(int dev, Kernel kernel, int threads, size_t smem, int size,
                                          tsds_cluster_counts& known) {
   int n = known[dev][size].load(std::memory_order_relaxed) - 1;   // 0: not asked yet
   if (n >= 0) return n;
+  std::lock_guard<std::mutex> hold(tsds_host_cache_lock());
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     cudaGetLastError();
     return 0;
@@ -145,7 +148,7 @@ static inline int tsds_resident_clusters(int dev, Kernel kernel, int threads, si
   cfg.numAttrs = 1;
   if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
     cudaGetLastError();
-    n = 0;
+    return 0;
   }
   known[dev][size].store(n + 1, std::memory_order_relaxed);
   return n;
