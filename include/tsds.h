@@ -263,7 +263,8 @@ int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const v
  * x: [M][K] bf16, A: [n_adapters][n_slices*R][K], B: [n_adapters][N][R],
  * contiguous.  n_slices projections side by side in y's columns (q, k, v:
  * 3): slice_widths (host array, each a multiple of 32, summing to N) gives
- * the columns of each, s(j) is column j's; NULL with one slice.  scale
+ * the columns of each, s(j) is column j's; one slice: NULL, or N, which need
+ * then not be a multiple of 32.  scale
  * (fp32) and ranks (int32, what an adapter uses of R; the rest of its A and
  * B is not part of the sum, whatever it holds) may be NULL: 1 and R.  The inner sum
  * is held as two bf16 words, infinities as they are; an infinity in B itself can

@@ -432,6 +432,8 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
       TSDS_RETURN_IF(at > N, TSDS_E_INVALID);
     }
     TSDS_RETURN_IF(at != N, TSDS_E_INVALID);
+  } else {
+    TSDS_RETURN_IF(slice_widths && slice_widths[0] != N, TSDS_E_INVALID);
   }
   p.first_col[n_slices] = N;
   if (M == 0) return TSDS_OK;
