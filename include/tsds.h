@@ -245,7 +245,7 @@ int tsds_add_rms_norm_fp8(const void* x, const void* res, const void* w, void* r
  *                              out = bf16(silu(acc_gate) * acc_up)
  * rounded once.  x: [M][K] e4m3 bytes (row stride ldx, ldx % 16 == 0), W
  * [n_out][K] e4m3 contiguous, K % 16 == 0, x and W 16-byte aligned; any M
- * and n_out.  tcgen05 tensor cores; no workspace.  *status (device int32,
+ * and K up to 2^30 and n_out up to 2^29.  tcgen05 tensor cores; no workspace.  *status (device int32,
  * zero before the first use): TSDS_E_TIMEOUT if a device wait gave up
  * (tsds_set_wait_limit_ns). */
 int tsds_linear_fp8(const void* x, int ldx, const float* x_scale, const void* W, const float* w_scale,
@@ -272,7 +272,8 @@ int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const v
  * out may be y (ldo == ldy; rows without an adapter are then not touched),
  * not x.  Beyond a few rows n_adapters * N < 2^31.
  * Any order of adapters; rows of one request next to one another are
- * fastest.  K % 8 == 0, N % 8 == 0, R % 8 == 0, R <= 128, n_slices <= 4;
+ * fastest.  K % 8 == 0, N % 8 == 0, R % 8 == 0, R <= 128, n_slices <= 4,
+ * 1 <= n_adapters, M <= 2^26, K and N <= 2^30;
  * strides multiples of 8, buffers 16-byte aligned.  An adapter[m] >= n_adapters is not
  * followed: the row is treated as one without and *status = TSDS_E_INDEX. */
 int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, const void* lora_a, const void* lora_b,

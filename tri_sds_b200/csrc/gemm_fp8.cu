@@ -740,6 +740,8 @@ int check(const void* x, int ldx, const float* sx, const void* w, const float* s
           int n_out, int K, const int32_t* status) {
   TSDS_RETURN_IF(M < 0 || n_out <= 0 || K <= 0 || (K % 16) != 0 || ldx < K || ldo < n_out || n_out > (1 << 29),
                  TSDS_E_INVALID);
+  // rows and K are rounded up to whole blocks in 32 bits
+  TSDS_RETURN_IF(M > (1 << 30) || K > (1 << 30), TSDS_E_UNSUPPORTED);
   if (M == 0) return TSDS_OK;
   TSDS_RETURN_IF(!x || !sx || !w || !sw || !out || !status, TSDS_E_INVALID);
   TSDS_RETURN_IF(!tsds_aligned16(x) || !tsds_aligned16(w) || (ldx % 16), TSDS_E_ALIGN);

@@ -419,7 +419,8 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
                      (R % 8) != 0 || ldx < K || ldy < N || ldo < N,
                  TSDS_E_INVALID);
   TSDS_RETURN_IF(n_slices < 1 || (n_slices > 1 && !slice_widths), TSDS_E_INVALID);
-  TSDS_RETURN_IF(R > MAX_RANK || n_slices > MAX_SLICES || M > (1 << 26), TSDS_E_UNSUPPORTED);
+  TSDS_RETURN_IF(R > MAX_RANK || n_slices > MAX_SLICES || M > (1 << 26) || K > (1 << 30) || N > (1 << 30),
+                 TSDS_E_UNSUPPORTED);
   LoraArgs p = {};
   p.S = n_slices;
   if (n_slices > 1) {

@@ -429,13 +429,19 @@ def _one_device(t, *ts) -> int:
     return dev
 
 
+_INT = 2 ** 31 - 1   # sizes and strides are 32-bit there; ctypes would cut them off without a word
+
+
 def _ld(t, rows: int, n: int, what: str) -> int:
     """The row stride of a [rows, n] buffer with unit inner stride (of one
     row: n, whatever torch keeps there)."""
     st = t.stride()
     if t.shape != (rows, n) or (st[1] != 1 and n > 1):
         raise ValueError(f"{what} must be [{rows}, {n}] with unit inner stride")
-    return st[0] if rows > 1 else n
+    ld = st[0] if rows > 1 else n
+    if rows > _INT or ld > _INT or n > _INT:
+        raise ValueError(f"{what}: rows, columns and row stride must be below 2^31")
+    return ld
 
 
 def _vec(t, n: int, what: str) -> None:
@@ -518,6 +524,7 @@ def _fp8_operands(x, x_scale, w, w_scale, n_out, out):
     M, K = x.shape
     if w.shape[1] != K or not w.is_contiguous():
         raise ValueError("w must be contiguous [out, K]")
+    _need(n_out <= _INT, "w: rows must be below 2^31")
     _vec(x_scale, M, "x_scale")
     _vec(w_scale, w.shape[0], "w_scale (a scale per row of w)")
     return M, K, *_bf16_output(x, M, n_out, out)
@@ -583,6 +590,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: tor
     if lora_a.shape != (n_ad, S * R, K) or lora_b.shape != (n_ad, N, R):
         raise ValueError(f"lora_a must be [adapters, {S * R}, {K}] and lora_b [adapters, {N}, R]")
     _need(lora_a.is_contiguous() and lora_b.is_contiguous(), "lora_a and lora_b must be contiguous")
+    _need(n_ad <= _INT and R <= _INT, "lora_a and lora_b: adapters and ranks must be below 2^31")
     _vec(adapter, M, "adapter")
     for t in (scale, ranks):
         if t is not None:
