@@ -223,7 +223,9 @@ int tsds_linear_bias(const void* x, int ldx, const void* W, const void* bias, vo
  *   or an infinity gets a NaN or infinite scale and NaN values.
  * x: [rows][n] bf16, row stride ldx; q: [rows][n] bytes, row stride ldq;
  * n % 16 == 0, ldx % 8 == 0, ldq % 16 == 0, x and q 16-byte aligned.
- * rows == 0 is allowed here and below (nothing is launched).
+ * rows == 0 is allowed here and below (nothing is launched).  Outputs that share bytes
+ * with what the call reads are refused here and below, but for those that
+ * each call names; columns of one wider buffer share none.
  */
 int tsds_quant_fp8(const void* x, void* q, float* scale, int rows, int n, int ldx, int ldq,
                    tsds_stream_t stream);
@@ -233,8 +235,8 @@ int tsds_quant_fp8(const void* x, void* q, float* scale, int rows, int n, int ld
  *   (q, scale) = the row quantisation of y as above
  *   norm_out = bf16(y)                   optional: what adapters beside the projection read
  * res NULL: r = x, res_out unused.  res_out (row stride ld_res_out) may be
- * res or x itself, with its row stride: the update in place.  Other overlaps
- * are not allowed.  Same alignment rules as above. */
+ * res or x itself, with its row stride: the update in place; so may norm_out,
+ * where res_out is not the same.  Same alignment rules as above. */
 int tsds_add_rms_norm_fp8(const void* x, const void* res, const void* w, void* res_out, void* q,
                           float* scale, void* norm_out, int rows, int n, int ldx, int ld_res,
                           int ld_res_out, int ldq, int ld_norm, float eps, tsds_stream_t stream);

@@ -89,3 +89,93 @@ def test_sizes_and_strides_past_32_bits_raise(monkeypatch):
         with pytest.raises(ValueError, match="below 2"):
             call()
             pytest.fail(f"case {i} was accepted")
+
+
+# -- outputs over what a call reads ---------------------------------------------------
+
+def quant(lib, x=FAR[0], q=FAR[1], s=FAR[2], rows=4, n=64, ldx=64, ldq=64):
+    return lib.tsds_quant_fp8(P(x), P(q), P(s), rows, n, ldx, ldq, None)
+
+
+def norm(lib, x=FAR[0], res=FAR[1], w=FAR[2], ro=FAR[3], q=FAR[4], s=FAR[5], no=FAR[6], rows=4, n=64, ldx=64, ldr=64,
+         ldo=64, ldq=64, ldn=64):
+    return lib.tsds_add_rms_norm_fp8(P(x), P(res), P(w), P(ro), P(q), P(s), P(no), rows, n, ldx, ldr, ldo, ldq, ldn, 1e-6,
+                                     None)
+
+
+def test_quantiser_over_its_input(lib):
+    x = FAR[0]
+    for bad in (dict(q=x), dict(q=x, ldq=128), dict(q=x + 64, ldq=128), dict(q=x - 16), dict(q=x + 128 * 3 + 112),
+                dict(q=x, rows=1), dict(q=x + 16, ldq=256, ldx=128), dict(q=x + 144, ldq=240, ldx=128, rows=9)):
+        assert quant(lib, **bad) == INVALID, bad
+
+
+def test_norm_outputs_over_one_another_and_operands(lib):
+    x, res, ro, q, no = FAR[0], FAR[1], FAR[3], FAR[4], FAR[6]
+    for bad in (dict(no=ro), dict(no=ro + 16), dict(no=ro - 16), dict(no=res, ro=res), dict(no=x, ro=x),
+                dict(q=x), dict(q=res), dict(q=ro), dict(q=no), dict(q=no + 128 * 3), dict(ro=res + 16), dict(ro=x - 16),
+                dict(no=x + 32), dict(no=res + 128), dict(no=x, ldn=72)):
+        assert norm(lib, **bad) == INVALID, bad
+    assert norm(lib, no=x, res=None, ro=None, q=x) == INVALID
+
+
+@pytest.mark.parametrize("kind", ["store", "residual", "swiglu"])
+def test_projection_output_over_its_operands(lib, kind):
+    x, w = FAR[0], FAR[2]
+    for bad in (dict(out=x), dict(out=x + 64), dict(out=x - 4), dict(out=w), dict(out=w + 32 * 64 - 2), dict(out=w - 126)):
+        assert linear(lib, kind, **bad) == INVALID, bad
+    if kind == "swiglu":
+        assert linear(lib, kind, out=w + 63 * 64) == INVALID     # 64 rows of gate and up
+    if kind == "residual":
+        for out in (FAR[6] + 2, FAR[6] - 2, FAR[6] + 64):
+            assert linear(lib, kind, out=out) == INVALID
+        assert linear(lib, kind, out=FAR[6] + 4, ldo=64, ldr=64) == INVALID
+
+
+def test_adapter_output_over_its_operands(lib):
+    y, x, a, b = FAR[0], FAR[1], FAR[2], FAR[3]
+    for M in (2, 2000):
+        for out in (x, x + 16, x - 16, y + 16, y - 16, y + 128, a, a + 2 * 16 * 64 * 2 - 16, b, b + 2 * 64 * 16 * 2 - 16):
+            assert lora(lib, out=out, M=M) == INVALID, (M, hex(out))
+
+
+# Row sets side by side, as a program that asks the same arithmetic of random ones would see them.
+OVERLAP = r"""
+#include <cstdio>
+#include "common.cuh"
+std::mutex& tsds_host_cache_lock() { static std::mutex m; return m; }
+void tsds_count_launch() {}
+int main() {
+  long long a[4], b[4];
+  while (std::scanf("%lld %lld %lld %lld %lld %lld %lld %lld", a, a + 1, a + 2, a + 3, b, b + 1, b + 2, b + 3) == 8)
+    std::printf("%d\n", (int)tsds_overlap({(void*)a[0], a[1], a[2], a[3]}, {(void*)b[0], b[1], b[2], b[3]}));
+}
+"""
+
+
+def test_overlap_of_random_row_sets(tmp_path):
+    """Against sets of bytes, same and different strides, interleaved columns among them."""
+    import os
+    import random
+    import subprocess
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src, exe = tmp_path / "overlap.cu", tmp_path / "overlap"
+    src.write_text(OVERLAP)
+    subprocess.run([nvcc, "-std=c++17", "-I", os.path.join(root, "tri_sds_b200", "csrc"), str(src), "-o", str(exe)],
+                   check=True, capture_output=True)
+    rng = random.Random(5)
+    cases, want = [], []
+    for _ in range(4000):
+        rows, ld = rng.randint(1, 6), rng.randint(1, 40)
+        sets = [(rng.randint(200, 420), r, s, rng.randint(1, s))
+                for r, s in ((rows, ld), (rng.choice([rows, rng.randint(1, 6)]), rng.choice([ld, ld, rng.randint(1, 40)])))]
+        cases.append(" ".join(str(v) for s in sets for v in s))
+        a, b = ({p + i * s + k for i in range(r) for k in range(w)} for p, r, s, w in sets)
+        want.append(int(bool(a & b)))
+    out = subprocess.run([str(exe)], input="\n".join(cases), capture_output=True, text=True, check=True).stdout.split()
+    bad = [(c, w) for c, w, g in zip(cases, want, out) if w != int(g)]
+    assert not bad, bad[:5]
+    assert 0 < sum(want) < len(want)

@@ -90,3 +90,34 @@ def test_norm_weights_made_just_before_the_call(ops):
             torch.cuda.synchronize()
             for gq, gs, _ in got:
                 assert torch.equal(gq.view(torch.uint8), q.view(torch.uint8)) and torch.equal(gs, s)
+
+
+def test_columns_of_one_buffer_side_by_side(ops):
+    """Operands and outputs as columns of the same wide rows share no byte and are served; norm_out over x or the
+    residual gives the values it gives elsewhere."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    M, n = 300, 256
+    wide = torch.randn(M, 5 * n, device=DEV, generator=g).to(BF)
+    x, r, ro, no, qb = (wide[:, i * n:(i + 1) * n] for i in range(5))
+    q = qb.view(E4M3)[:, :n]
+    w = torch.randn(n, device=DEV, generator=g).to(BF)
+    x0, r0 = x.clone(), r.clone()
+    want_no = torch.empty(M, n, device=DEV, dtype=BF)
+    want = ops.add_rms_norm_fp8(x0, w, residual=r0, norm_out=want_no)
+    s = torch.empty(M, device=DEV)
+    ops.add_rms_norm_fp8(x, w, residual=r, res_out=ro, norm_out=no, out=q, scale=s)
+    assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+    assert torch.equal(ro, want[2]) and torch.equal(no, want_no) and torch.equal(x, x0) and torch.equal(r, r0)
+    wq, ws = ops.quant_fp8(torch.randn(n, n, device=DEV, generator=g).to(BF))
+    proj = ops.linear_residual_fp8(q, s, wq, ws, r)
+    ops.linear_residual_fp8(q, s, wq, ws, r, out=no)
+    assert torch.equal(no, proj)
+    for n in (256, 40000):
+        x0, r0 = torch.randn(9, n, device=DEV, generator=g).to(BF), torch.randn(9, n, device=DEV, generator=g).to(BF)
+        w, no = torch.randn(n, device=DEV, generator=g).to(BF), torch.empty(9, n, device=DEV, dtype=BF)
+        want = ops.add_rms_norm_fp8(x0, w, residual=r0, norm_out=no)
+        for over in range(2):
+            xr = [x0.clone(), r0.clone()]
+            got = ops.add_rms_norm_fp8(xr[0], w, residual=xr[1], norm_out=xr[over])
+            assert torch.equal(xr[over], no) and torch.equal(got[2], want[2]) and torch.equal(got[1], want[1])
+            assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))

@@ -31,6 +31,36 @@ static inline int tsds_launch_status() {
 
 static inline bool tsds_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Rows of `width` bytes, `ld` bytes apart.
+struct tsds_rows {
+  const void* base;
+  int64_t rows, ld, width;
+};
+
+// Whether two sets of rows share a byte (host arithmetic on the addresses).  Columns of
+// one wider buffer, which interleave without sharing any, are told apart by their
+// offset where both have the same stride, else row by row.
+static inline bool tsds_overlap(const tsds_rows& a, const tsds_rows& b) {
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.base), b0 = reinterpret_cast<uintptr_t>(b.base);
+  if (!a0 || !b0 || a.rows <= 0 || b.rows <= 0) return false;
+  const uintptr_t a1 = a0 + (a.rows - 1) * a.ld + a.width, b1 = b0 + (b.rows - 1) * b.ld + b.width;
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (a.ld == b.ld && a.rows > 1 && b.rows > 1) {
+    const int64_t d = (int64_t)(b0 - a0) % a.ld, at = d < 0 ? d + a.ld : d;   // b's first column in a's rows
+    return at < a.width || at + b.width > a.ld;
+  }
+  for (int64_t i = 0, j = 0; i < a.rows && j < b.rows;) {
+    const uintptr_t p = a0 + i * a.ld, q = b0 + j * b.ld;
+    if (p + a.width <= q)
+      ++i;
+    else if (q + b.width <= p)
+      ++j;
+    else
+      return true;
+  }
+  return false;
+}
+
 // Host-side state of the library is safe under calls from several host
 // threads at once (the ABI allows concurrent calls on different streams):
 // per-device "done" records are atomics, and the small lookup caches of

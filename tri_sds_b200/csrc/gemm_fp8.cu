@@ -736,8 +736,9 @@ int run(const uint8_t* x, int ldx, const uint8_t* w, F8Args p, int K, cudaStream
                  : launch<EPI, 1, false>(amap, bmap, p, grid, smem, stream);
 }
 
-int check(const void* x, int ldx, const float* sx, const void* w, const float* sw, const void* out, int ldo, int M,
-          int n_out, int K, const int32_t* status) {
+// w_rows: rows of W
+int check(const void* x, int ldx, const float* sx, const void* w, int64_t w_rows, const float* sw, const void* out,
+          int ldo, int M, int n_out, int K, const int32_t* status) {
   TSDS_RETURN_IF(M < 0 || n_out <= 0 || K <= 0 || (K % 16) != 0 || ldx < K || ldo < n_out || n_out > (1 << 29),
                  TSDS_E_INVALID);
   // rows and K are rounded up to whole blocks in 32 bits
@@ -745,6 +746,9 @@ int check(const void* x, int ldx, const float* sx, const void* w, const float* s
   if (M == 0) return TSDS_OK;
   TSDS_RETURN_IF(!x || !sx || !w || !sw || !out || !status, TSDS_E_INVALID);
   TSDS_RETURN_IF(!tsds_aligned16(x) || !tsds_aligned16(w) || (ldx % 16), TSDS_E_ALIGN);
+  // (a block's rows are stored while others still read theirs)
+  const tsds_rows o = {out, M, ldo * (int64_t)2, n_out * (int64_t)2};
+  TSDS_RETURN_IF(tsds_overlap(o, {x, M, ldx, K}) || tsds_overlap(o, {w, 1, 0, w_rows * K}), TSDS_E_INVALID);
   return TSDS_OK;
 }
 
@@ -764,7 +768,7 @@ F8Args args_of(const float* sx, const float* sw, void* out, int ldo, int M, int 
 
 extern "C" int tsds_linear_fp8(const void* x, int ldx, const float* x_scale, const void* W, const float* w_scale,
                                void* out, int ldo, int M, int n_out, int K, int32_t* status, tsds_stream_t stream) {
-  const int st = check(x, ldx, x_scale, W, w_scale, out, ldo, M, n_out, K, status);
+  const int st = check(x, ldx, x_scale, W, n_out, w_scale, out, ldo, M, n_out, K, status);
   if (st != TSDS_OK || M == 0) return st;
   return run<EPI_STORE>((const uint8_t*)x, ldx, (const uint8_t*)W,
                         args_of(x_scale, w_scale, out, ldo, M, n_out, status), K, stream);
@@ -773,11 +777,14 @@ extern "C" int tsds_linear_fp8(const void* x, int ldx, const float* x_scale, con
 extern "C" int tsds_linear_residual_fp8(const void* x, int ldx, const float* x_scale, const void* W,
                                         const float* w_scale, const void* res, int res_ld, void* out, int ldo, int M,
                                         int n_out, int K, int32_t* status, tsds_stream_t stream) {
-  const int st = check(x, ldx, x_scale, W, w_scale, out, ldo, M, n_out, K, status);
+  const int st = check(x, ldx, x_scale, W, n_out, w_scale, out, ldo, M, n_out, K, status);
   if (st != TSDS_OK) return st;
   TSDS_RETURN_IF(res_ld < n_out, TSDS_E_INVALID);
   if (M == 0) return TSDS_OK;
   TSDS_RETURN_IF(!res || (res == out && res_ld != ldo), TSDS_E_INVALID);
+  TSDS_RETURN_IF(res != out && tsds_overlap({out, M, ldo * (int64_t)2, n_out * (int64_t)2},
+                                            {res, M, res_ld * (int64_t)2, n_out * (int64_t)2}),
+                 TSDS_E_INVALID);
   F8Args p = args_of(x_scale, w_scale, out, ldo, M, n_out, status);
   p.res = (const bf16*)res;
   p.res_ld = res_ld;
@@ -787,7 +794,7 @@ extern "C" int tsds_linear_residual_fp8(const void* x, int ldx, const float* x_s
 extern "C" int tsds_linear_swiglu_fp8(const void* x, int ldx, const float* x_scale, const void* W,
                                       const float* w_scale, void* out, int ldo, int M, int n_out, int K,
                                       int32_t* status, tsds_stream_t stream) {
-  const int st = check(x, ldx, x_scale, W, w_scale, out, ldo, M, n_out, K, status);
+  const int st = check(x, ldx, x_scale, W, 2 * (int64_t)n_out, w_scale, out, ldo, M, n_out, K, status);
   if (st != TSDS_OK || M == 0) return st;
   return run<EPI_SWIGLU>((const uint8_t*)x, ldx, (const uint8_t*)W,
                          args_of(x_scale, w_scale, out, ldo, M, n_out, status), K, stream);

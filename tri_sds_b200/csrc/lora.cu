@@ -442,7 +442,6 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   TSDS_RETURN_IF(!tsds_aligned16(y) || !tsds_aligned16(x) || !tsds_aligned16(lora_a) || !tsds_aligned16(lora_b) ||
                      !tsds_aligned16(out) || (ldx % 8) || (ldy % 8) || (ldo % 8),
                  TSDS_E_ALIGN);
-  // x is read while out is written
   TSDS_RETURN_IF((out == y && ldo != ldy) || out == x, TSDS_E_INVALID);
   p.x = (const bf16*)x;
   p.y = (const bf16*)y;
@@ -464,13 +463,21 @@ extern "C" int tsds_lora_add(const void* y, int ldy, const void* x, int ldx, con
   // rows of t: 16 elements past a multiple of 64, so that the fragments'
   // 8-byte reads of four rows cover all banks
   p.ld_t = (n_slices * ((R + 15) / 16 * 16) + 63) / 64 * 64 + 16;
-  if (!few_rows(M, K, R, n_slices, n_adapters)) {
+  const bool few = few_rows(M, K, R, n_slices, n_adapters);
+  if (!few) {
     // rows of A and B are tensor-map coordinates there
     TSDS_RETURN_IF((int64_t)n_adapters * (N > n_slices * R ? N : n_slices * R) > 0x7fffffff, TSDS_E_UNSUPPORTED);
     TSDS_RETURN_IF(!workspace || workspace_bytes < tsds_lora_tc_workspace_bytes(M, R, n_slices), TSDS_E_WORKSPACE);
     TSDS_RETURN_IF(!tsds_aligned16(workspace), TSDS_E_ALIGN);
-    return tsds_lora_tc(p, workspace, stream);
   }
+  // what is read while out is written: everything but y, and y too unless each element is out's own
+  const int64_t r = (int64_t)n_adapters * R * 2;
+  const tsds_rows o = {out, M, ldo * (int64_t)2, N * (int64_t)2};
+  TSDS_RETURN_IF(tsds_overlap(o, {x, M, ldx * (int64_t)2, K * (int64_t)2}) ||
+                     (out != y && tsds_overlap(o, {y, M, ldy * (int64_t)2, N * (int64_t)2})) ||
+                     tsds_overlap(o, {lora_a, 1, 0, r * n_slices * K}) || tsds_overlap(o, {lora_b, 1, 0, r * N}),
+                 TSDS_E_INVALID);
+  if (!few) return tsds_lora_tc(p, workspace, stream);
   // Where a cluster for every adapter of every tile fits the SMs at once the call
   // is a matter of latency: many warps and loads per CTA (q/k/v adapters of 8
   // one-token requests 10.8 us, 14.2 with the smaller CTAs).  With more of them two

@@ -235,6 +235,14 @@ int launch_rows(const QuantArgs& a, int rows, cudaStream_t stream) {
   return launch<NORM, 512, 8>(a, rows, stream);
 }
 
+tsds_rows rows_bf16(const void* p, int rows, int ld, int n) { return {p, rows, ld * (int64_t)2, n * (int64_t)2}; }
+
+// Whether an output may lie where it does beside a bf16 operand of the same rows: apart from it, or
+// exactly on it.
+bool apart_or_same(const tsds_rows& out, const tsds_rows& in) {
+  return (out.base == in.base && out.ld == in.ld) || !tsds_overlap(out, in);
+}
+
 }  // namespace
 
 extern "C" int tsds_quant_fp8(const void* x, void* q, float* scale, int rows, int n, int ldx, int ldq,
@@ -243,6 +251,8 @@ extern "C" int tsds_quant_fp8(const void* x, void* q, float* scale, int rows, in
   if (rows == 0) return TSDS_OK;
   TSDS_RETURN_IF(!x || !q || !scale, TSDS_E_INVALID);
   TSDS_RETURN_IF(!tsds_aligned16(x) || !tsds_aligned16(q) || (ldx % 8) || (ldq % 16), TSDS_E_ALIGN);
+  // (a long row is read twice, the second time after its first bytes are written)
+  TSDS_RETURN_IF(tsds_overlap({q, rows, ldq, n}, rows_bf16(x, rows, ldx, n)), TSDS_E_INVALID);
   QuantArgs a = {};
   a.x = (const bf16*)x;
   a.q = (uint8_t*)q;
@@ -267,6 +277,13 @@ extern "C" int tsds_add_rms_norm_fp8(const void* x, const void* res, const void*
   TSDS_RETURN_IF(res && ((res_out == res && ld_res_out != ld_res) || (res_out == x && ld_res_out != ldx)),
                  TSDS_E_INVALID);
   TSDS_RETURN_IF(norm_out && (!tsds_aligned16(norm_out) || (ld_norm % 8)), TSDS_E_ALIGN);
+  const tsds_rows rx = rows_bf16(x, rows, ldx, n), rr = rows_bf16(res, rows, ld_res, n),
+                  ro = rows_bf16(res ? res_out : nullptr, rows, ld_res_out, n),
+                  rn = rows_bf16(norm_out, rows, ld_norm, n), rq = {q, rows, ldq, n};
+  TSDS_RETURN_IF(tsds_overlap(rq, rx) || tsds_overlap(rq, rr) || tsds_overlap(rq, ro) || tsds_overlap(rq, rn) ||
+                     tsds_overlap(rn, ro) || !apart_or_same(ro, rx) || !apart_or_same(ro, rr) ||
+                     !apart_or_same(rn, rx) || !apart_or_same(rn, rr),
+                 TSDS_E_INVALID);
   QuantArgs a = {};
   a.x = (const bf16*)x;
   a.res = (const bf16*)res;

@@ -493,7 +493,8 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     one launch: (q [rows, n] float8_e4m3fn, scale [rows] fp32, res_out [rows,
     n] bf16).  res_out may be the residual itself (the update in place).
     Without a residual r = x and res_out is None.  norm_out, when given,
-    receives y in bf16 (what per-request adapters read, see lora_add)."""
+    receives y in bf16 (what per-request adapters read, see lora_add); it may
+    be x or the residual, but not where res_out is."""
     _bf16_cuda(x, weight, residual, res_out, norm_out)
     _need(x.dim() == 2, "x must be [rows, n]")
     rows, n = x.shape
