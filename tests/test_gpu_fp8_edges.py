@@ -121,3 +121,39 @@ def test_columns_of_one_buffer_side_by_side(ops):
             got = ops.add_rms_norm_fp8(xr[0], w, residual=xr[1], norm_out=xr[over])
             assert torch.equal(xr[over], no) and torch.equal(got[2], want[2]) and torch.equal(got[1], want[1])
             assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
+
+
+@pytest.mark.parametrize("kind,M,n,K", [("residual", 208, 5120, 25600), ("store", 200, 10240, 5120), ("swiglu", 208, 25600, 5120),
+                                        ("residual", 700, 5120, 8192)])
+def test_wait_limit_of_cta_pairs_reports_and_recovers(ops, kind, M, n, K):
+    """Above 128 rows two CTAs work on a unit: their waits run out at any moment of a call, the call ends, says so, and
+    the next one is right."""
+    from tri_sds_b200 import _lib
+    lib = _lib.load()
+    g = torch.Generator(device=DEV).manual_seed(M + n)
+    xq, xs = ops.quant_fp8(torch.randn(M, K, device=DEV, generator=g).to(BF))
+    wq, ws = ops.quant_fp8(torch.randn(2 * n if kind == "swiglu" else n, K, device=DEV, generator=g).to(BF))
+    res = torch.randn(M, n, device=DEV, generator=g).to(BF)
+
+    def call():
+        if kind == "residual":
+            return ops.linear_residual_fp8(xq, xs, wq, ws, res)
+        return (ops.linear_fp8 if kind == "store" else ops.linear_swiglu_fp8)(xq, xs, wq, ws)
+    want = call()
+    ops.check_status()
+    limit = lib.tsds_get_wait_limit_ns()
+    for ns in (1, 500, 2000, 5000, 10000, 20000):
+        try:
+            lib.tsds_set_wait_limit_ns(ns)
+            got = call()
+            torch.cuda.synchronize()
+        finally:
+            lib.tsds_set_wait_limit_ns(limit)
+        try:
+            ops.check_status()
+            assert torch.equal(got, want)    # every wait was met after all
+            assert ns > 1
+        except RuntimeError as e:
+            assert "timed out" in str(e)
+        assert torch.equal(call(), want)
+        ops.check_status()

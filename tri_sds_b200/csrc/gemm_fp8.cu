@@ -72,6 +72,7 @@ struct F8Shared {
   uint64_t full[RING], empty[RING], tfull[2], tempty[2], drain;
   uint32_t tmem;
   int abort;
+  int given_up, peer_issued;   // pairs: a CTA of the cluster gave up; blocks that the leader's peer requested
 };
 
 template <int CG>
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
       mbar_init(&sh.tempty[i], 4 * CG);   // one arrival per epilogue warp
     }
     mbar_init(&sh.drain, 1);
-    sh.abort = 0;
+    sh.abort = sh.given_up = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -490,8 +491,8 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
   tc_fence_after();
   const bool alive = !*(volatile int*)&sh.abort;
   if (!alive) {  // uniform: copies and MMAs in flight finish (bounded) before TMEM is freed
-    // (a pair's land on the leader's barriers; the other CTA leaves after it)
-    if (warp == 0 && lane == 0 && half == 0) drain_tma_ring(sh.full, p.stages, issued);
+    // (a pair's copies at the end, when neither CTA requests any more)
+    if (CG == 1 && warp == 0 && lane == 0) drain_tma_ring(sh.full, p.stages, issued);
     if (warp == 1 && lane == 0 && issued > 0) {
       commit<CG>(&sh.drain, pair);
       mbar_wait(&sh.drain, 0, 20000000ull);
@@ -571,8 +572,27 @@ __global__ void __launch_bounds__(THREADS, SPLIT || CG == 2 ? 1 : 3)
     }
   }
   tc_fence_before();
+  if constexpr (CG == 2) {
+    if (!alive && threadIdx.x < p.C * CG) st_peer(mapa_shared(smem_u32(&sh.given_up), threadIdx.x), 1);
+  }
   __syncthreads();
-  if constexpr (CG == 2) cluster_barrier();   // the pair is done with both TMEM halves and barriers
+  if constexpr (CG == 2) {
+    cluster_barrier();   // the pair is done with both TMEM halves and barriers
+    if (*(volatile int*)&sh.given_up) {
+      // (the same in every CTA of the cluster)  A pair's copies all land on the leader's
+      // barriers, but each CTA requested its own: what the peer requested beyond the
+      // leader's count is expected now, so that the drain waits for it too.  What it
+      // requested less never comes, and costs the drain its limit.
+      if (half == 1 && warp == 0 && lane == 0) st_peer(mapa_shared(smem_u32(&sh.peer_issued), lead), issued);
+      cluster_barrier();
+      if (half == 0 && warp == 0 && lane == 0) {
+        const int peer = *(volatile int*)&sh.peer_issued;
+        for (int j = issued; j < peer; ++j) mbar_arrive_expect_tx(&sh.full[j % p.stages], A_BYTES + p.b_bytes);
+        drain_tma_ring(sh.full, p.stages, peer > issued ? peer : issued);
+      }
+      cluster_barrier();
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CG == 2)

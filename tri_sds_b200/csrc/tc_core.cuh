@@ -95,6 +95,10 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ void st_peer(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 // ---- stream-K bookkeeping ---------------------------------------------------
 // 32-bit arithmetic: W * P < 2^32 is checked on the host.
 __device__ __forceinline__ int it_begin(int p, int P, uint32_t W) { return (int)(((uint32_t)p * W) / (uint32_t)P); }
