@@ -92,3 +92,51 @@ def test_adapter_written_just_before_the_call(ops, M):
     torch.cuda.synchronize()
     for i, o in enumerate(got):
         assert torch.equal(o, want[i % 3]), i
+
+
+FIRST = r"""
+import sys
+import torch
+sys.path.insert(0, REPO)
+from tri_sds_b200 import ops
+y, x = torch.ones(4, 64, device="cuda").bfloat16(), torch.ones(4, 64, device="cuda").bfloat16()
+a, b = torch.ones(2, 8, 64, device="cuda").bfloat16(), torch.ones(2, 64, 8, device="cuda").bfloat16()
+good = torch.zeros(4, device="cuda", dtype=torch.int32)
+bad = torch.full((4,), 7, device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+graphs = []
+for ids in (good, bad):          # the process's first calls
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.lora_add(y, x, a, b, ids)
+    graphs.append((graph, out))
+ops.check_status()
+graphs[0][0].replay()
+torch.cuda.synchronize()
+assert (graphs[0][1] == 1 + 8 * 64).all()
+ops.check_status()
+graphs[1][0].replay()
+graphs[0][0].replay()            # a later replay leaves the report alone
+try:
+    ops.check_status()
+except RuntimeError as e:
+    assert "status 10" in str(e)
+else:
+    raise SystemExit("the report of an index past the last adapter was lost")
+graphs[1][0].replay()
+ops.lora_add(y, x, a, b, good)
+try:
+    ops.check_status()
+except RuntimeError:
+    print("reported")
+ops.check_status()
+"""
+
+
+def test_status_of_a_process_whose_first_calls_are_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST.replace("REPO", repr(root))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "reported" in r.stdout, r.stdout + r.stderr

@@ -80,9 +80,21 @@ class _Scratch:
         key = torch.device(device).index
         s = self.status.get(key)
         if s is None:
-            s = torch.zeros(1, dtype=torch.int32, device=device)
-            self.status[key] = s
+            s = self.status[key] = self._zero_word(torch.device(device))
         return s
+
+    @staticmethod
+    def _zero_word(device) -> torch.Tensor:
+        if device.type != "cuda":
+            return torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                return torch.zeros(1, dtype=torch.int32, device=device)
+            # the first call of all is being captured: zeroed here and now on a stream of its
+            # own, or each replay of that graph would zero it and lose what others reported
+            word = torch.empty(1, dtype=torch.int32, device=device)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                return word.zero_()
 
 
 _scratch = _Scratch()
