@@ -157,3 +157,51 @@ def test_wait_limit_of_cta_pairs_reports_and_recovers(ops, kind, M, n, K):
             assert "timed out" in str(e)
         assert torch.equal(call(), want)
         ops.check_status()
+
+
+def _norm_tolerance(rows, n):
+    """What the scale of a normalised row may be off by: the longest chain of additions of its squares (a thread's
+    vectors of 8, five steps within a warp, the warps one after another; each off by 2^-24 of the sum, which the root
+    halves together with the mean's and eps's rounding), then root, reciprocal, the product with the largest
+    value and the division by 448."""
+    if n <= 8192:
+        threads = 256
+    elif rows < 2 * 148 or n > 32768:
+        threads = 1024
+    else:
+        threads = 512
+    additions = 8 * -(-(n // 8) // threads) + 5 + threads // 32
+    return ((additions + 2) / 2 + 4) * ref.F32 * (1 + 2.0 ** -10)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 16), (26, 5120), (3, 8192), (601, 8208), (601, 16384), (601, 16400), (601, 32768),
+                                    (601, 32784), (2, 12288), (5, 32768), (2, 40000), (2, 262144)])
+def test_norm_scales_within_their_additions(ops, rows, n):
+    g = torch.Generator(device=DEV).manual_seed(rows + n)
+    x, r = (torch.randn(rows, n, device=DEV, generator=g).to(BF) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(n, device=DEV, generator=g)).to(BF)
+    q, s, ro = ops.add_rms_norm_fp8(x, w, residual=r)
+    assert torch.equal(ro, (x.float() + r.float()).to(BF))
+    ref.check_quant(q, s, _norm_values(ro, w, 1e-6), _norm_tolerance(rows, n))
+
+
+@pytest.mark.parametrize("kind", ["store", "residual", "swiglu"])
+@pytest.mark.parametrize("M,n,K", [(208, 1280, 5120), (40, 333, 528)])
+def test_rows_of_a_batch_on_their_own(ops, kind, M, n, K):
+    """A request's rows alone and inside a batch: other launch shapes, the same definition."""
+    g = torch.Generator(device=DEV).manual_seed(M)
+    xq, xs = ops.quant_fp8(torch.randn(M, K, device=DEV, generator=g).to(BF))
+    wq, ws = ops.quant_fp8(torch.randn(2 * n if kind == "swiglu" else n, K, device=DEV, generator=g).to(BF))
+    res = torch.randn(M, n, device=DEV, generator=g).to(BF)
+    acc, err = ref.linear(xq, xs, wq, ws)
+    if kind == "residual":
+        acc, err = acc + res.double(), err + ref.F32 * (acc.abs() + res.double().abs())
+    elif kind == "swiglu":
+        acc, err = ref.silu_mul(acc[:, :n], err[:, :n], acc[:, n:], err[:, n:])
+    for lo, hi in ((0, M), (0, 1), (M - 1, M), (7, 33), (3, 36)):
+        a = (xq[lo:hi], xs[lo:hi], wq, ws)
+        if kind == "residual":
+            got = ops.linear_residual_fp8(*a, res[lo:hi])
+        else:
+            got = (ops.linear_fp8 if kind == "store" else ops.linear_swiglu_fp8)(*a)
+        ref.check_bf16(got, acc[lo:hi], err[lo:hi])
