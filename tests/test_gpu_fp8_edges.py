@@ -205,3 +205,27 @@ def test_rows_of_a_batch_on_their_own(ops, kind, M, n, K):
         else:
             got = (ops.linear_fp8 if kind == "store" else ops.linear_swiglu_fp8)(*a)
         ref.check_bf16(got, acc[lo:hi], err[lo:hi])
+
+
+def _exact_quant(x):
+    """Rows of bf16 to the nearest e4m3 of x * 448 / max|x|, ties to even, without a rounding: |x| * 448 and a
+    midpoint times max|x| have at most 17 and 13 significant bits, so fp64 compares them exactly."""
+    a = x.double().abs()
+    top = a.amax(dim=1, keepdim=True)
+    v = a * ref.TOP / top * (1 - 2.0 ** -50)      # never above the value's grid cell
+    step = ref.e4m3_step(v)
+    lo = torch.floor(v / step)
+    num, mid = a * ref.TOP, (lo + 0.5) * step * top
+    up = (num > mid) | ((num == mid) & (lo % 2 == 1))
+    return torch.copysign((lo + up) * step, x.double())
+
+
+@pytest.mark.parametrize("rows,n", [(26, 25600), (1000, 5120), (513, 8208), (3, 32784)])
+def test_quantiser_is_exact(ops, rows, n):
+    """Every value, on rows with a few channels tens of times larger as a residual stream has them."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.randn(rows, n, device=DEV, generator=g)
+    x[:, torch.randint(0, n, (n // 512,), device=DEV, generator=g)] *= 30.0
+    x = x.to(BF)
+    q, _ = ops.quant_fp8(x)
+    assert torch.equal(q.double(), _exact_quant(x))
