@@ -49,7 +49,8 @@ constexpr int RANKS = 64;     // columns of t, at most: 8 n8 tiles
 // rows of one adapter, rank 16 in three 15.2 and 15.5, rank 16 in one 13.1 and 13.7, rank
 // 32 in one 16.7 and 14.1, 1024 rows 24.2 and 18.4; 128 rows that alternate between 16
 // adapters, rank 16 in one 44 and 29.  K 25600 -> 5120: 8 rows, rank 16 10.3 and 21.3;
-// 208 rows, rank 48 28.8 and 21.3; 512 rows, rank 64 42.8 and 21.3.
+// 208 rows, rank 48 28.8 and 21.3; 512 rows, rank 64 42.8 and 21.3.  (Taken with read-only loads of A
+// and B; with the plain ones the first case takes 10.1 us here, 8 x 26 rows 14.2 and 13.8.)
 bool few_rows(int M, int K, int R, int S, int n_adapters) {
   const int tiles = (M + TR - 1) / TR, SR = S * R;
   if (M > 512 || tiles * (n_adapters < TR ? n_adapters : TR) > 104) return false;

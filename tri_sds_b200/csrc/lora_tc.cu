@@ -16,13 +16,14 @@
 //
 // The bytes of x and y bound both (B and A come from L2 after their first
 // use); the MMAs are a few percent of the tensor cores' rate.  2048 rows, K 5120,
-// rank 32 into q/k/v of 10240 columns: 30.4 us, shrink about 13 of them (21 MB of x, the
+// rank 32 into q/k/v of 10240 columns: 30.0 us, shrink about 13 of them (21 MB of x, the
 // rest the chain from launch to reduction) and expand 17 (84 MB of y and out,
 // 5 TB/s).  Asking for y from shrink already, into L2, cost 7 us.
 //
 // shrink lets its successor start only after its own dependency wait, so
 // everything before shrink is complete when expand begins, and expand may
-// read y, B and the indices before its wait; only t comes after it.
+// read y, B and the indices before its wait; only t comes after it.  With one CTA of expand
+// per SM that starts where shrink has left an SM: their shared memory does not fit together.
 #include "common.cuh"
 #include "linear.cuh"
 #include "lora.cuh"
@@ -669,9 +670,9 @@ int tsds_lora_tc(const LoraArgs& l, void* workspace, cudaStream_t stream) {
   p.ld_t = l.S * p.Rp;
   // Token rows per shrink block: 32 for few rows (more clusters; 8 x 26 rows at
   // rank 64 into q/k/v 23.6 us, with 64 26.2), 64 above (an adapter's A is read
-  // less often; 16 x 26 rows, K 25600, rank 16 26 us, with 32 37), 128 where
-  // that still makes two CTAs per SM (4096 rows at rank 16 into q/k/v 47.7 us, with 64
-  // 52.7; 2048 rows at rank 32 32.3 and 30.4)
+  // less often; 16 x 26 rows, K 25600, rank 16 26 us, with 32 37), 128 from 3584 rows on,
+  // where even one adapter per block makes 28 clusters, 1.5 CTAs per SM (4096 rows at
+  // rank 16 into q/k/v 47.7 us, with 64 52.7; 2048 rows, 16 clusters, at rank 32 32.3 and 30.4)
   p.nt = l.M <= 256 ? 32 : (l.M < 3584 ? 64 : 128);
   p.blocks = (l.M + p.nt - 1) / p.nt;
   const int SR = l.S * l.R;

@@ -18,7 +18,7 @@
 //
 // A row stays in one CTA's registers, so each of its bytes moves once and HBM
 // bounds many rows: 10240 rows of 5120 quantised in 25.4 us (6.2 TB/s), 4096 rows
-// of 5120 with residual, norm and both outputs in 29.9 us (6.3 TB/s).  Few rows are a
+// of 5120 with residual, norm and both outputs in 30.0 us (6.3 TB/s).  Few rows are a
 // launch, the row's loads and the CTA's two reductions: 26 rows of 25600 in 2.8 us.
 #include "common.cuh"
 #include "linear.cuh"
